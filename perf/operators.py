@@ -309,7 +309,8 @@ def _plan(st):
         rows, vocab = st["logits"].shape
         out = torch.empty_like(st["logits"])
         call = kc.KernelCall.LogitRules(kc.LogitRulesCall(
-            ref(st["logits"]), ref(st["history"]), ref(st["spans"]), ref(st["params"]), ref(st["bias_starts"]), ref(st["bias_ids"]), ref(st["bias_values"]), ref(st["masks"]),
+            ref(st["logits"]), ref(st["history"]), ref(st["spans"]), ref(st["params"]),
+            ref(st["bias_starts"] if case["bias"] else None), ref(st["bias_ids"]), ref(st["bias_values"]), ref(st["masks"]),
             ref(st["mask_of"]), ref(out), rows, vocab, vocab, vocab, st["history"].shape[1], st["bias_ids"].numel(), 0 if st["masks"] is None else 4, (vocab + 31) // 32,
             tag))
     else:
