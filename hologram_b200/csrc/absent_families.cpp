@@ -1,5 +1,5 @@
 // Stands in for the kernel families a serving build leaves out (LUT activations, the reference-exact matmul and decode
-// attention, quantized products, tensor parallelism): a call that needs one is refused.
+// attention, packed sequences and block caches, quantized products, tensor parallelism): a call that needs one is refused.
 #include "common.h"
 
 namespace {
@@ -22,6 +22,9 @@ int32_t holo_launch_matmul_e8cb_omajor(holo_b200_ctx*, const float*, const uint8
                                        uint32_t, uint32_t, int) { return absent("quantized product"); }
 int32_t holo_launch_matmul_w8a8_omajor(holo_b200_ctx*, const float*, const int8_t*, const float*, const int32_t*, const float*, float*, uint32_t, uint32_t, uint32_t,
                                        int, bool) { return absent("quantized product"); }
+int32_t holo_launch_packed_attention(holo_b200_ctx*, const HoloPackedArgs&) { return absent("packed attention"); }
+int32_t holo_launch_block_cache_write(holo_b200_ctx*, const HoloBlockWriteArgs&) { return absent("block cache"); }
+int32_t holo_launch_block_cache_attention(holo_b200_ctx*, const HoloBlockAttnArgs&) { return absent("block cache"); }
 int32_t holo_all_reduce(holo_b200_ctx*, void*, uint64_t, uint8_t) { return absent("tensor-parallel"); }
 int32_t holo_all_reduce_add(holo_b200_ctx*, const void*, const void*, void*, uint64_t, uint8_t) { return absent("tensor-parallel"); }
 void holo_tp_destroy(holo_b200_ctx*) {}

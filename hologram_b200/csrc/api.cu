@@ -145,6 +145,8 @@ static int32_t check_dev_status(holo_b200_ctx* ctx, void* host = nullptr, const 
     cudaMemsetAsync(ctx->dev_status, 0, 4, ctx->stream);
     if (st & 2u) cudaMemsetAsync(ctx->attn_arrivals, 0, 65536 * 4, ctx->stream);  // a launch that gave up may have left counts behind
     if (st & 1u) return holo_fail_slot(HOLO_NO_SLOT, "gather index outside [−axis_dim, axis_dim)");
+    if (st & HOLO_STATUS_TABLE)
+        return holo_fail(HOLO_ERR_DISPATCH, "dispatch failed: a call's starts, lengths, block numbers, spans or mask numbers on the device are out of range (status 0x%x)", st);
     return holo_fail(HOLO_ERR_DISPATCH, "dispatch failed: a device-side bounded wait gave up (status 0x%x)", st);
 }
 
@@ -1315,6 +1317,152 @@ int32_t do_moe_combine(holo_b200_ctx* ctx, const HoloMoeCombineCall& c, holo_b20
     return holo_launch_moe_combine(ctx, (float*)x, y, (const float*)weight, (const int32_t*)place, (const uint32_t*)step, c.rows, c.width, c.top, c.ld, c.y_rows, c.dtype);
 }
 
+// ---- a serving step over several sequences (all extensions) ----
+// 0 selects 1 / sqrt(dim); a scale that is not positive would turn the running maximum into a minimum.
+int32_t score_scale(const char* what, uint32_t scale_bits, uint32_t dim, float* scale) {
+    *scale = scale_bits ? f32_of_bits(scale_bits) : 1.0f / sqrtf((float)dim);
+    if (!(*scale > 0.0f) || *scale > 3.0e38f) return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: %s: the scale must be positive and finite", what);
+    return HOLO_OK;
+}
+
+int32_t do_packed_attention(holo_b200_ctx* ctx, const HoloPackedAttentionCall& c, holo_b200_workspace* ws) {
+    if (!holo_is_compute_float(c.dtype)) return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: packed_attention dtype %u", c.dtype);
+    if (c.rows == 0 || c.sequences == 0 || c.heads == 0) return HOLO_OK;
+    if (c.kv_heads == 0 || c.heads % c.kv_heads != 0)
+        return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: packed_attention: heads must be a multiple of kv_heads (grouped-query)");
+    if (c.dim == 0 || c.vdim == 0 || c.dim > 512 || c.vdim > 512 || c.rows > 0x7fffffffu || c.sequences > 0x7ffffffeu)
+        return holo_fail(HOLO_ERR_SHAPE_MISMATCH, "shape mismatch: packed_attention dim %u, vdim %u, %u rows", c.dim, c.vdim, c.rows);
+    const uint64_t es = holo_dtype_size(c.dtype);
+    HoloPackedArgs a = {};
+    HOLO_TRY(score_scale("packed_attention", c.scale_bits, c.dim, &a.scale));
+    uint8_t *q, *k, *v, *starts, *out;
+    Range rq, rk, rv, ro;
+    HOLO_TRY(resolve_rows(ws, c.q, c.rows, c.q_ld, (uint64_t)c.heads * c.dim, es, &q, &rq));
+    HOLO_TRY(resolve_rows(ws, c.k, c.rows, c.k_ld, (uint64_t)c.kv_heads * c.dim, es, &k, &rk));
+    HOLO_TRY(resolve_rows(ws, c.v, c.rows, c.v_ld, (uint64_t)c.kv_heads * c.vdim, es, &v, &rv));
+    HOLO_TRY(resolve_words(ws, c.starts, c.sequences + 1ull, &starts));
+    HOLO_TRY(resolve_rows(ws, c.output, c.rows, c.ld, (uint64_t)c.heads * c.vdim, es, &out, &ro));
+    HOLO_TRY(check_disjoint(ro, c.output.slot, {rq, rk, rv, {starts, 4 * (c.sequences + 1ull)}}));
+    a.q = q; a.k = k; a.v = v; a.starts = (const int32_t*)starts; a.out = out;
+    a.rows = c.rows; a.sequences = c.sequences; a.heads = c.heads; a.kv_heads = c.kv_heads; a.dim = c.dim; a.vdim = c.vdim;
+    a.q_ld = c.q_ld; a.k_ld = c.k_ld; a.v_ld = c.v_ld; a.ld = c.ld;
+    a.dtype = c.dtype;
+    a.causal = c.causal != 0;
+    a.status = ctx->dev_status;
+    return holo_launch_packed_attention(ctx, a);
+}
+
+// The operands of an int8 block cache. `r`: starts, lengths, table, k codes, k scales, v codes, v scales.
+template <typename Call>
+int32_t resolve_block_cache(holo_b200_ctx* ctx, holo_b200_workspace* ws, const char* what, const Call& c, HoloBlockCache* out, Range (&r)[7]) {
+    if (c.kv_heads == 0 || c.dim == 0 || c.vdim == 0 || c.dim > 512 || c.vdim > 512 || c.block_rows == 0 || c.block_rows > 1024 || c.table_ld == 0 || c.blocks == 0 ||
+        c.blocks > 0x7fffffffu || c.rows > 0x7fffffffu || c.sequences > 0x7ffffffeu || (uint64_t)c.table_ld * c.block_rows > 0x7fffffffull)
+        return holo_fail(HOLO_ERR_SHAPE_MISMATCH, "shape mismatch: %s dim %u, vdim %u, %u blocks of %u rows, %u a sequence", what, c.dim, c.vdim, c.blocks, c.block_rows, c.table_ld);
+    const bool singles = c.starts.slot == HOLO_NO_SLOT;
+    if (singles && c.rows != c.sequences)
+        return holo_fail(HOLO_ERR_SHAPE_MISMATCH, "shape mismatch: %s without starts has a row a sequence: %u rows, %u sequences", what, c.rows, c.sequences);
+    const uint64_t planes = (uint64_t)c.blocks * c.kv_heads, kb = planes * c.block_rows * c.dim, vb = planes * c.block_rows * c.vdim;
+    uint8_t *starts = nullptr, *lengths, *table, *kc, *ks, *vc, *vs;
+    if (!singles) HOLO_TRY(resolve_words(ws, c.starts, c.sequences + 1ull, &starts));
+    HOLO_TRY(resolve_words(ws, c.lengths, c.sequences, &lengths));
+    HOLO_TRY(resolve_words(ws, c.table, (uint64_t)c.sequences * c.table_ld, &table));
+    HOLO_TRY(holo_resolve(ws, c.k_codes, kb, &kc, nullptr));
+    HOLO_TRY(resolve_words(ws, c.k_scales, planes, &ks));
+    HOLO_TRY(holo_resolve(ws, c.v_codes, vb, &vc, nullptr));
+    HOLO_TRY(resolve_words(ws, c.v_scales, planes, &vs));
+    const Range ranges[7] = {{starts, singles ? 0 : 4 * (c.sequences + 1ull)}, {lengths, 4ull * c.sequences}, {table, 4ull * c.sequences * c.table_ld},
+                             {kc, kb}, {ks, 4 * planes}, {vc, vb}, {vs, 4 * planes}};
+    for (int i = 0; i < 7; ++i) r[i] = ranges[i];
+    out->starts = (const int32_t*)starts; out->lengths = (const int32_t*)lengths; out->table = (const int32_t*)table;
+    out->k_codes = (int8_t*)kc; out->k_scales = (float*)ks; out->v_codes = (int8_t*)vc; out->v_scales = (float*)vs;
+    out->rows = c.rows; out->sequences = c.sequences; out->kv_heads = c.kv_heads; out->dim = c.dim; out->vdim = c.vdim;
+    out->block_rows = c.block_rows; out->blocks = c.blocks; out->table_ld = c.table_ld;
+    out->status = ctx->dev_status;
+    return HOLO_OK;
+}
+
+int32_t do_block_cache_write(holo_b200_ctx* ctx, const HoloBlockCacheWriteCall& c, holo_b200_workspace* ws) {
+    if (!holo_is_compute_float(c.dtype)) return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: block_cache_write dtype %u", c.dtype);
+    if (c.rows == 0 || c.sequences == 0) return HOLO_OK;
+    const uint64_t es = holo_dtype_size(c.dtype);
+    HoloBlockWriteArgs a = {};
+    Range r[7], rk, rv;
+    uint8_t *k, *v;
+    HOLO_TRY(resolve_block_cache(ctx, ws, "block_cache_write", c, &a.c, r));
+    HOLO_TRY(resolve_rows(ws, c.k, c.rows, c.k_ld, (uint64_t)c.kv_heads * c.dim, es, &k, &rk));
+    HOLO_TRY(resolve_rows(ws, c.v, c.rows, c.v_ld, (uint64_t)c.kv_heads * c.vdim, es, &v, &rv));
+    const HoloBufferRef written[4] = {c.k_codes, c.k_scales, c.v_codes, c.v_scales};
+    for (int i = 3; i < 7; ++i) {
+        HOLO_TRY(check_disjoint(r[i], written[i - 3].slot, {rk, rv, r[0], r[1], r[2]}));
+        for (int j = 3; j < i; ++j) HOLO_TRY(check_disjoint(r[i], written[i - 3].slot, {r[j]}));
+    }
+    a.k = k; a.v = v; a.k_ld = c.k_ld; a.v_ld = c.v_ld;
+    a.dtype = c.dtype;
+    return holo_launch_block_cache_write(ctx, a);
+}
+
+int32_t do_block_cache_attention(holo_b200_ctx* ctx, const HoloBlockCacheAttentionCall& c, holo_b200_workspace* ws) {
+    if (!holo_is_compute_float(c.dtype)) return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: block_cache_attention dtype %u", c.dtype);
+    if (c.rows == 0 || c.sequences == 0 || c.heads == 0) return HOLO_OK;
+    if (c.kv_heads == 0 || c.heads % c.kv_heads != 0)
+        return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: block_cache_attention: heads must be a multiple of kv_heads (grouped-query)");
+    const uint64_t es = holo_dtype_size(c.dtype);
+    HoloBlockAttnArgs a = {};
+    Range r[7], rq, ro;
+    uint8_t *q, *out;
+    HOLO_TRY(resolve_block_cache(ctx, ws, "block_cache_attention", c, &a.c, r));
+    HOLO_TRY(score_scale("block_cache_attention", c.scale_bits, c.dim, &a.scale));
+    HOLO_TRY(resolve_rows(ws, c.q, c.rows, c.q_ld, (uint64_t)c.heads * c.dim, es, &q, &rq));
+    HOLO_TRY(resolve_rows(ws, c.output, c.rows, c.ld, (uint64_t)c.heads * c.vdim, es, &out, &ro));
+    HOLO_TRY(check_disjoint(ro, c.output.slot, {rq, r[0], r[1], r[2], r[3], r[4], r[5], r[6]}));
+    a.q = q; a.out = out; a.heads = c.heads; a.q_ld = c.q_ld; a.ld = c.ld;
+    a.dtype = c.dtype;
+    return holo_launch_block_cache_attention(ctx, a);
+}
+
+int32_t do_logit_rules(holo_b200_ctx* ctx, const HoloLogitRulesCall& c, holo_b200_workspace* ws) {
+    if (!holo_is_compute_float(c.dtype)) return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: logit_rules dtype %u", c.dtype);
+    if (c.rows == 0 || c.vocab == 0) return HOLO_OK;
+    auto has = [](const HoloBufferRef& r) { return r.slot != HOLO_NO_SLOT; };
+    const bool history = has(c.history), bias = has(c.bias_ids), mask = has(c.masks);
+    if (c.vocab > 0x7fffffffu || c.rows > 0x7fffffffu || (history && (c.history_ld == 0 || c.history_ld > 0x7fffffffu)) || (bias && (c.biases == 0 || c.biases > 0x7fffffffu)) ||
+        (mask && (c.mask_rows == 0 || c.mask_ld < (c.vocab + 31) / 32)) || (mask && !has(c.mask_of) && c.mask_rows < c.rows))
+        return holo_fail(HOLO_ERR_SHAPE_MISMATCH, "shape mismatch: logit_rules of %u tokens, history %u, %u biases, %u masks of %u words", c.vocab, c.history_ld, c.biases,
+                         c.mask_rows, c.mask_ld);
+    if (history != has(c.spans) || bias != has(c.bias_starts) || bias != has(c.bias_values) || (has(c.mask_of) && !mask) || (history && !has(c.params)))
+        return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: logit_rules: history comes with spans and params, bias_ids with bias_starts and bias_values, mask_of with masks");
+    const uint64_t es = holo_dtype_size(c.dtype);
+    uint8_t *z, *out, *hist = nullptr, *spans = nullptr, *params = nullptr, *bs = nullptr, *bi = nullptr, *bv = nullptr, *masks = nullptr, *mask_of = nullptr;
+    Range rz, ro;
+    HOLO_TRY(resolve_rows(ws, c.logits, c.rows, c.ld, c.vocab, es, &z, &rz));
+    HOLO_TRY(resolve_rows(ws, c.output, c.rows, c.out_ld, c.vocab, es, &out, &ro));
+    const uint64_t nh = (uint64_t)c.rows * c.history_ld, nm = (uint64_t)c.mask_rows * c.mask_ld;
+    if (history) {
+        HOLO_TRY(resolve_words(ws, c.history, nh, &hist));
+        HOLO_TRY(resolve_words(ws, c.spans, 2ull * c.rows, &spans));
+    }
+    if (has(c.params)) HOLO_TRY(resolve_words(ws, c.params, 4ull * c.rows, &params));
+    if (bias) {
+        HOLO_TRY(resolve_words(ws, c.bias_starts, c.rows + 1ull, &bs));
+        HOLO_TRY(resolve_words(ws, c.bias_ids, c.biases, &bi));
+        HOLO_TRY(resolve_words(ws, c.bias_values, c.biases, &bv));
+    }
+    if (mask) HOLO_TRY(resolve_words(ws, c.masks, nm, &masks));
+    if (has(c.mask_of)) HOLO_TRY(resolve_words(ws, c.mask_of, c.rows, &mask_of));
+    // in place: every thread reads its own logits before it stores them
+    if (!(z == out && c.ld == c.out_ld)) HOLO_TRY(check_disjoint(ro, c.output.slot, {rz}));
+    HOLO_TRY(check_disjoint(ro, c.output.slot, {{hist, hist ? 4 * nh : 0}, {spans, spans ? 8ull * c.rows : 0}, {params, params ? 16ull * c.rows : 0},
+                                                {bs, bs ? 4 * (c.rows + 1ull) : 0}, {bi, bi ? 4ull * c.biases : 0}, {bv, bv ? 4ull * c.biases : 0},
+                                                {masks, masks ? 4 * nm : 0}, {mask_of, mask_of ? 4ull * c.rows : 0}}));
+    HoloLogitRulesArgs a = {};
+    a.logits = z; a.out = out; a.history = (const int32_t*)hist; a.spans = (const int32_t*)spans; a.params = (const float*)params;
+    a.bias_starts = (const int32_t*)bs; a.bias_ids = (const int32_t*)bi; a.bias_values = (const float*)bv; a.masks = (const uint32_t*)masks; a.mask_of = (const int32_t*)mask_of;
+    a.rows = c.rows; a.vocab = c.vocab; a.ld = c.ld; a.out_ld = c.out_ld; a.history_ld = c.history_ld; a.biases = c.biases; a.mask_rows = c.mask_rows; a.mask_ld = c.mask_ld;
+    a.dtype = c.dtype;
+    a.status = ctx->dev_status;
+    return holo_launch_logit_rules(ctx, a);
+}
+
 int32_t do_all_reduce(holo_b200_ctx* ctx, const HoloAllReduceCall& c, holo_b200_workspace* ws) {
     size_t es = holo_dtype_size(c.dtype);
     if (c.dtype != HOLO_DTYPE_F32 && c.dtype != HOLO_DTYPE_BF16 && c.dtype != HOLO_DTYPE_F16)
@@ -1383,6 +1531,10 @@ int32_t holo_dispatch_internal(holo_b200_ctx* ctx, const HoloKernelCall* call, h
         case HOLO_K_MOE_PLAN: return do_moe_plan(ctx, call->u.moe_plan, ws);
         case HOLO_K_MOE_COMBINE: return do_moe_combine(ctx, call->u.moe_combine, ws);
         case HOLO_K_CAUSAL_ATTENTION: return do_causal_attention(ctx, call->u.causal_attention, ws);
+        case HOLO_K_PACKED_ATTENTION: return do_packed_attention(ctx, call->u.packed_attention, ws);
+        case HOLO_K_BLOCK_CACHE_WRITE: return do_block_cache_write(ctx, call->u.block_cache_write, ws);
+        case HOLO_K_BLOCK_CACHE_ATTENTION: return do_block_cache_attention(ctx, call->u.block_cache_attention, ws);
+        case HOLO_K_LOGIT_RULES: return do_logit_rules(ctx, call->u.logit_rules, ws);
         default:
             if (holo_is_exact_unary(call->kind) || holo_is_exact_binary(call->kind)) return do_elementwise(ctx, call, ws);
             return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: KernelCall variant %u is not served by the B200 backend (no CPU fallback)", call->kind);
@@ -1619,6 +1771,33 @@ bool holo_collect_refs(HoloKernelCall* c, HoloRefList* l) {
             l->out(&q.x, 4ull * q.rows * q.width);
             return true;
         }
+        case HOLO_K_PACKED_ATTENTION: {
+            auto& q = c->u.packed_attention;
+            l->in(&q.q); l->in(&q.k); l->in(&q.v); l->in(&q.starts);
+            l->out(&q.output, ((uint64_t)(q.rows - 1) * q.ld + (uint64_t)q.heads * q.vdim) * holo_dtype_size(q.dtype));
+            return true;
+        }
+        case HOLO_K_BLOCK_CACHE_WRITE: {
+            auto& q = c->u.block_cache_write;
+            const uint64_t planes = (uint64_t)q.blocks * q.kv_heads;
+            l->in(&q.k); l->in(&q.v); l->in(&q.starts); l->in(&q.lengths); l->in(&q.table);
+            l->out(&q.k_codes, planes * q.block_rows * q.dim); l->out(&q.k_scales, 4 * planes);
+            l->out(&q.v_codes, planes * q.block_rows * q.vdim); l->out(&q.v_scales, 4 * planes);
+            return true;
+        }
+        case HOLO_K_BLOCK_CACHE_ATTENTION: {
+            auto& q = c->u.block_cache_attention;
+            l->in(&q.q); l->in(&q.starts); l->in(&q.lengths); l->in(&q.table); l->in(&q.k_codes); l->in(&q.k_scales); l->in(&q.v_codes); l->in(&q.v_scales);
+            l->out(&q.output, ((uint64_t)(q.rows - 1) * q.ld + (uint64_t)q.heads * q.vdim) * holo_dtype_size(q.dtype));
+            return true;
+        }
+        case HOLO_K_LOGIT_RULES: {
+            auto& q = c->u.logit_rules;
+            l->in(&q.logits); l->in(&q.history); l->in(&q.spans); l->in(&q.params); l->in(&q.bias_starts); l->in(&q.bias_ids); l->in(&q.bias_values);
+            l->in(&q.masks); l->in(&q.mask_of);
+            l->out(&q.output, ((uint64_t)(q.rows - 1) * q.out_ld + q.vocab) * holo_dtype_size(q.dtype));
+            return true;
+        }
         case HOLO_K_CAUSAL_ATTENTION: {
             auto& q = c->u.causal_attention;
             l->in(&q.q); l->in(&q.k); l->in(&q.v); l->in(&q.pos); l->in(&q.sink);
@@ -1648,7 +1827,7 @@ extern "C" int32_t holo_b200_dispatch_host(holo_b200_ctx* ctx, const HoloKernelC
     HoloRefList refs;
     bool appends = false;   // rows of a cache at a device-side position: only a device-resident buffer has them
     // the buffers these keep from call to call (caches, state, residual) are device-resident as well
-    if (call->kind >= HOLO_K_LINEAR_EX && call->kind <= HOLO_K_MOE_COMBINE) appends = true;
+    if (call->kind >= HOLO_K_LINEAR_EX && call->kind <= HOLO_K_LOGIT_RULES) appends = true;
     if (call->kind == HOLO_K_LINEAR)
         for (uint32_t i = 0; i < call->u.linear.nseg && i < HOLO_LINEAR_MAX_SEGS; ++i) appends |= call->u.linear.seg[i].row_pos.slot != HOLO_NO_SLOT;
     if (appends || !holo_collect_refs(&local, &refs))

@@ -304,6 +304,39 @@ int32_t decode_call(Reader& r, HoloKernelCall* out) {
             if (c.rows == 0) return holo_fail(HOLO_ERR_INIT, "backend init failed: combination over no rows");
             break;
         }
+        case HOLO_K_PACKED_ATTENTION: {
+            HoloPackedAttentionCall& c = out->u.packed_attention;
+            for (HoloBufferRef* b : {&c.q, &c.k, &c.v, &c.starts, &c.output}) *b = r.buf();
+            for (uint32_t* f : {&c.rows, &c.sequences, &c.heads, &c.kv_heads, &c.dim, &c.vdim, &c.q_ld, &c.k_ld, &c.v_ld, &c.ld, &c.scale_bits}) *f = r.u32();
+            c.causal = r.u8(); c.dtype = r.u8();
+            if (c.rows == 0) return holo_fail(HOLO_ERR_INIT, "backend init failed: packed attention over no rows");
+            break;
+        }
+        case HOLO_K_BLOCK_CACHE_WRITE: {
+            HoloBlockCacheWriteCall& c = out->u.block_cache_write;
+            for (HoloBufferRef* b : {&c.k, &c.v, &c.starts, &c.lengths, &c.table, &c.k_codes, &c.k_scales, &c.v_codes, &c.v_scales}) *b = r.buf();
+            for (uint32_t* f : {&c.rows, &c.sequences, &c.kv_heads, &c.dim, &c.vdim, &c.k_ld, &c.v_ld, &c.block_rows, &c.blocks, &c.table_ld}) *f = r.u32();
+            c.dtype = r.u8();
+            if (c.rows == 0) return holo_fail(HOLO_ERR_INIT, "backend init failed: block cache write of no rows");
+            break;
+        }
+        case HOLO_K_BLOCK_CACHE_ATTENTION: {
+            HoloBlockCacheAttentionCall& c = out->u.block_cache_attention;
+            for (HoloBufferRef* b : {&c.q, &c.starts, &c.lengths, &c.table, &c.k_codes, &c.k_scales, &c.v_codes, &c.v_scales, &c.output}) *b = r.buf();
+            for (uint32_t* f : {&c.rows, &c.sequences, &c.heads, &c.kv_heads, &c.dim, &c.vdim, &c.q_ld, &c.ld, &c.block_rows, &c.blocks, &c.table_ld, &c.scale_bits})
+                *f = r.u32();
+            c.dtype = r.u8();
+            if (c.rows == 0) return holo_fail(HOLO_ERR_INIT, "backend init failed: block cache attention over no rows");
+            break;
+        }
+        case HOLO_K_LOGIT_RULES: {
+            HoloLogitRulesCall& c = out->u.logit_rules;
+            for (HoloBufferRef* b : {&c.logits, &c.history, &c.spans, &c.params, &c.bias_starts, &c.bias_ids, &c.bias_values, &c.masks, &c.mask_of, &c.output}) *b = r.buf();
+            for (uint32_t* f : {&c.rows, &c.vocab, &c.ld, &c.out_ld, &c.history_ld, &c.biases, &c.mask_rows, &c.mask_ld}) *f = r.u32();
+            c.dtype = r.u8();
+            if (c.rows == 0) return holo_fail(HOLO_ERR_INIT, "backend init failed: logit rules over no rows");
+            break;
+        }
         case HOLO_K_CAUSAL_ATTENTION: {
             HoloCausalAttentionCall& c = out->u.causal_attention;
             c.q = r.buf(); c.k = r.buf(); c.v = r.buf(); c.pos = r.buf(); c.sink = r.buf(); c.output = r.buf();

@@ -390,6 +390,59 @@ struct HoloMoePlanArgs {
 int32_t holo_launch_moe_plan(holo_b200_ctx* ctx, const HoloMoePlanArgs& a);
 int32_t holo_launch_moe_combine(holo_b200_ctx* ctx, float* x, const void* y, const float* weight, const int32_t* place, const uint32_t* step, uint32_t rows,
                                 uint32_t width, uint32_t top, uint32_t ld, uint32_t y_rows, uint8_t dtype);
+// packed_attention.cu
+struct HoloPackedArgs {
+    const void *q, *k, *v;
+    const int32_t* starts;
+    void* out;
+    uint32_t rows, sequences, heads, kv_heads, dim, vdim, q_ld, k_ld, v_ld, ld;
+    float scale;
+    uint8_t dtype;
+    bool causal;
+    uint32_t* status;
+};
+int32_t holo_launch_packed_attention(holo_b200_ctx* ctx, const HoloPackedArgs& a);
+// block_cache.cu: the cache's operands, shared by its two calls
+struct HoloBlockCache {
+    const int32_t *starts, *lengths, *table;     // starts null: row s is sequence s's only one
+    int8_t *k_codes, *v_codes;
+    float *k_scales, *v_scales;
+    uint32_t rows, sequences, kv_heads, dim, vdim, block_rows, blocks, table_ld;
+    uint32_t* status;
+};
+struct HoloBlockWriteArgs {
+    HoloBlockCache c;
+    const void *k, *v;
+    uint32_t k_ld, v_ld;
+    uint8_t dtype;
+};
+int32_t holo_launch_block_cache_write(holo_b200_ctx* ctx, const HoloBlockWriteArgs& a);
+struct HoloBlockAttnArgs {
+    HoloBlockCache c;
+    const void* q;
+    void* out;
+    uint32_t heads, q_ld, ld;
+    float scale;
+    uint8_t dtype;
+};
+int32_t holo_launch_block_cache_attention(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a);
+// logit_rules.cu
+struct HoloLogitRulesArgs {
+    const void* logits;
+    const int32_t *history, *spans;
+    const float* params;
+    const int32_t *bias_starts, *bias_ids;
+    const float* bias_values;
+    const uint32_t* masks;
+    const int32_t* mask_of;
+    void* out;
+    uint32_t rows, vocab, ld, out_ld, history_ld, biases, mask_rows, mask_ld;
+    uint8_t dtype;
+    uint32_t* status;
+};
+int32_t holo_launch_logit_rules(holo_b200_ctx* ctx, const HoloLogitRulesArgs& a);
+// bits of the status word: what a kernel found out of range on the device
+constexpr uint32_t HOLO_STATUS_TABLE = 8u;
 // quant_gemv.cu
 int32_t holo_launch_matmul_e8cb_omajor(holo_b200_ctx* ctx, const float* a, const uint8_t* bq, const int8_t* codebook, const float* scales,
                                        const int32_t* zero_points, const float* residual, float* out, uint32_t m, uint32_t k, uint32_t n, int act);

@@ -773,7 +773,7 @@ int32_t holo_session_load_impl(holo_b200_ctx* ctx, const uint8_t* archive, uint6
     if (s->addressed) {
         // the labels of an addressed walk do not see rows written into a resident cache
         for (const HoloKernelCall& c : s->calls) {
-            if (c.kind >= HOLO_K_LINEAR_EX && c.kind <= HOLO_K_MOE_COMBINE) {
+            if (c.kind >= HOLO_K_LINEAR_EX && c.kind <= HOLO_K_LOGIT_RULES) {
                 delete s;
                 return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: an addressed session has no resident state (call %u)", c.kind);
             }

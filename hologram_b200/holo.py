@@ -32,7 +32,8 @@ def _matmul(c):
 
 # calls whose payload is written field by field as the struct lists them
 _FLAT = {kc.K_ROTARY_TABLE: "rotary_table", kc.K_HEAD_LINEAR: "head_linear", kc.K_WINDOW_ATTENTION: "window_attention", kc.K_RETENTION: "retention",
-         kc.K_MOE_PLAN: "moe_plan", kc.K_MOE_COMBINE: "moe_combine"}
+         kc.K_MOE_PLAN: "moe_plan", kc.K_MOE_COMBINE: "moe_combine", kc.K_PACKED_ATTENTION: "packed_attention",
+         kc.K_BLOCK_CACHE_WRITE: "block_cache_write", kc.K_BLOCK_CACHE_ATTENTION: "block_cache_attention", kc.K_LOGIT_RULES: "logit_rules"}
 
 
 def _flat(c):

@@ -43,6 +43,7 @@ K_ROPE_QUANTIZE_ROWS_I8 = 0x8004
 K_RMS_NORM_MULTI, K_LINEAR, K_CAUSAL_ATTENTION = 0x8005, 0x8006, 0x8007
 K_LINEAR_EX, K_ROTARY_TABLE, K_RMS_NORM_PARTS, K_HEAD_LINEAR = 0x8008, 0x8009, 0x800a, 0x800b
 K_WINDOW_ATTENTION, K_RETENTION, K_MOE_PLAN, K_MOE_COMBINE = 0x800c, 0x800d, 0x800e, 0x800f
+K_PACKED_ATTENTION, K_BLOCK_CACHE_WRITE, K_BLOCK_CACHE_ATTENTION, K_LOGIT_RULES = 0x8010, 0x8011, 0x8012, 0x8013
 LUT_KIND = {LUT_SIGMOID: K_SIGMOID, LUT_TANH: K_TANH, LUT_GELU: K_GELU, LUT_SILU: K_SILU, LUT_EXP: K_EXP, LUT_ERF: K_ERF}
 
 NO_SLOT = 0xFFFFFFFF
@@ -389,6 +390,30 @@ class MoeCombineCall(C.Structure):
         "rows", "width", "top", "ld", "y_rows")] + [("dtype", C.c_uint8)]
 
 
+class PackedAttentionCall(C.Structure):
+    """Extension: attention of whole sequences of different lengths, packed one behind another."""
+    _fields_ = [(n, BufferRef) for n in ("q", "k", "v", "starts", "output")] + [(n, C.c_uint32) for n in (
+        "rows", "sequences", "heads", "kv_heads", "dim", "vdim", "q_ld", "k_ld", "v_ld", "ld", "scale_bits")] + [("causal", C.c_uint8), ("dtype", C.c_uint8)]
+
+
+class BlockCacheWriteCall(C.Structure):
+    """Extension: key and value rows into a cache of int8 blocks, one scale for each block and head."""
+    _fields_ = [(n, BufferRef) for n in ("k", "v", "starts", "lengths", "table", "k_codes", "k_scales", "v_codes", "v_scales")] + [(n, C.c_uint32) for n in (
+        "rows", "sequences", "kv_heads", "dim", "vdim", "k_ld", "v_ld", "block_rows", "blocks", "table_ld")] + [("dtype", C.c_uint8)]
+
+
+class BlockCacheAttentionCall(C.Structure):
+    """Extension: attention of single tokens or portions of several sequences over the int8 block cache."""
+    _fields_ = [(n, BufferRef) for n in ("q", "starts", "lengths", "table", "k_codes", "k_scales", "v_codes", "v_scales", "output")] + [(n, C.c_uint32) for n in (
+        "rows", "sequences", "heads", "kv_heads", "dim", "vdim", "q_ld", "ld", "block_rows", "blocks", "table_ld", "scale_bits")] + [("dtype", C.c_uint8)]
+
+
+class LogitRulesCall(C.Structure):
+    """Extension: penalties for repeated tokens, biases, a temperature and grammar masks on logits."""
+    _fields_ = [(n, BufferRef) for n in ("logits", "history", "spans", "params", "bias_starts", "bias_ids", "bias_values", "masks", "mask_of", "output")] + [
+        (n, C.c_uint32) for n in ("rows", "vocab", "ld", "out_ld", "history_ld", "biases", "mask_rows", "mask_ld")] + [("dtype", C.c_uint8)]
+
+
 class _Payload(C.Union):
     _fields_ = [("unary", UnaryCall), ("binary", BinaryCall), ("matmul", MatMulCall),
                 ("matmul_activation", MatMulActivationCall), ("matmul_add", MatMulAddCall), ("matmul_add_activation", MatMulAddActivationCall), ("matmul_dequant", MatMulDequantCall), ("norm", NormCall),
@@ -400,7 +425,8 @@ class _Payload(C.Union):
                 ("rope_quantize", RopeQuantizeCall), ("rms_norm_multi", RmsNormMultiCall), ("linear", LinearCall),
                 ("causal_attention", CausalAttentionCall), ("rotary_table", RotaryTableCall), ("rms_norm_parts", RmsNormPartsCall),
                 ("head_linear", HeadLinearCall), ("window_attention", WindowAttentionCall), ("retention", RetentionCall),
-                ("moe_plan", MoePlanCall), ("moe_combine", MoeCombineCall)]
+                ("moe_plan", MoePlanCall), ("moe_combine", MoeCombineCall), ("packed_attention", PackedAttentionCall),
+                ("block_cache_write", BlockCacheWriteCall), ("block_cache_attention", BlockCacheAttentionCall), ("logit_rules", LogitRulesCall)]
 
 
 class KernelCall(C.Structure):
@@ -532,6 +558,14 @@ class KernelCall(C.Structure):
     def MoePlan(cls, c): return cls.of(K_MOE_PLAN, c)
     @classmethod
     def MoeCombine(cls, c): return cls.of(K_MOE_COMBINE, c)
+    @classmethod
+    def PackedAttention(cls, c): return cls.of(K_PACKED_ATTENTION, c)
+    @classmethod
+    def BlockCacheWrite(cls, c): return cls.of(K_BLOCK_CACHE_WRITE, c)
+    @classmethod
+    def BlockCacheAttention(cls, c): return cls.of(K_BLOCK_CACHE_ATTENTION, c)
+    @classmethod
+    def LogitRules(cls, c): return cls.of(K_LOGIT_RULES, c)
 
 
 KernelCall._FIELD = {
@@ -543,6 +577,8 @@ KernelCall._FIELD = {
     RmsNormMultiCall: "rms_norm_multi", LinearCall: "linear", CausalAttentionCall: "causal_attention",
     RotaryTableCall: "rotary_table", RmsNormPartsCall: "rms_norm_parts", HeadLinearCall: "head_linear", WindowAttentionCall: "window_attention",
     RetentionCall: "retention", MoePlanCall: "moe_plan", MoeCombineCall: "moe_combine",
+    PackedAttentionCall: "packed_attention", BlockCacheWriteCall: "block_cache_write", BlockCacheAttentionCall: "block_cache_attention",
+    LogitRulesCall: "logit_rules",
 }
 
 

@@ -160,6 +160,15 @@ extern "C" {
 #define HOLO_K_RETENTION 0x800d
 #define HOLO_K_MOE_PLAN 0x800e
 #define HOLO_K_MOE_COMBINE 0x800f
+/* A serving step over several sequences at once:
+ * PACKED_ATTENTION is attention of whole prompts of different lengths that lie one behind another;
+ * BLOCK_CACHE_WRITE puts key and value rows into a cache of int8 blocks with one scale for each block and head;
+ * BLOCK_CACHE_ATTENTION is attention of single tokens or portions of the sequences over that cache;
+ * LOGIT_RULES applies penalties for repeated tokens, biases, a temperature and grammar masks to logits. */
+#define HOLO_K_PACKED_ATTENTION 0x8010
+#define HOLO_K_BLOCK_CACHE_WRITE 0x8011
+#define HOLO_K_BLOCK_CACHE_ATTENTION 0x8012
+#define HOLO_K_LOGIT_RULES 0x8013
 
 /* BufferRef (crates/hologram-compute/src/workspace.rs:16-24). length == 0 means "the slot's
  * full extent from offset". slot == UINT32_MAX marks an absent optional operand
@@ -559,6 +568,71 @@ typedef struct HoloMoeCombineCall {
     uint8_t dtype;
 } HoloMoeCombineCall;
 
+/* Extension. Attention of whole sequences packed one behind another: sequence s is rows [starts[s], starts[s + 1]) of q, k, v and
+ * output (starts i32 [sequences + 1], ascending, from 0 to `rows` at most; empty sequences are allowed). Query head h reads kv head
+ * h / (heads / kv_heads). Row i sees the rows j <= i of its sequence (causal) or all of them. Scores and sums are f32:
+ *   out[i, h] = sum_j exp(scale q_i . k_j) v_j / sum_j exp(scale q_i . k_j)
+ * q [rows, heads * dim] with pitch q_ld, k [rows, kv_heads * dim] with pitch k_ld, v [rows, kv_heads * vdim] with pitch v_ld, output
+ * [rows, heads * vdim] with pitch ld, all `dtype` (f32, bf16 or f16; rounded to nearest), dims up to 512. scale_bits 0 selects
+ * 1 / sqrt(dim); another scale is positive and finite. Rows of no sequence are left as they were, a row whose scores are all -inf is
+ * zero. A row is a function of the rows it sees alone: what stands in others, infinities and NaN included, does not reach it.
+ * Starts that descend or leave [0, rows] are reported at the next synchronising call; rows outside any proper range are not stored. */
+typedef struct HoloPackedAttentionCall {
+    HoloBufferRef q, k, v, starts, output;
+    uint32_t rows, sequences, heads, kv_heads, dim, vdim, q_ld, k_ld, v_ld, ld, scale_bits;
+    uint8_t causal, dtype;
+} HoloPackedAttentionCall;
+
+/* The int8 block cache of the two calls below: codes i8 [blocks, kv_heads, block_rows, dim (k) or vdim (v)], scales f32 [blocks,
+ * kv_heads] each for k and v; the value held is code * scale. table i32 [sequences, table_ld]: position p of sequence s is row
+ * p % block_rows of block table[s, p / block_rows]. lengths i32 [sequences]: the positions of each sequence, those of the call's rows
+ * included. The call's rows are packed: sequence s has rows [starts[s], starts[s + 1]), which are its last positions (starts absent:
+ * row s is the one row of sequence s, and `rows` is `sequences`). Entries of the table behind a sequence's positions are not read.
+ * A block number outside [0, blocks), starts that descend or leave [0, rows] and lengths below a sequence's number of rows or above
+ * table_ld * block_rows are reported at the next synchronising call; nothing is read or written outside the buffers for them. */
+
+/* Extension. k [rows, kv_heads * dim] (pitch k_ld) and v [rows, kv_heads * vdim] (pitch v_ld), `dtype` f32, bf16 or f16, into the
+ * cache, after which lengths hold. For each block and head touched, m the largest finite magnitude of its new rows:
+ *   scale' = max(scale, m / 127)   (m / 127 where the block's first position is new),
+ *   code = the integer nearest to x / scale' (ties to even) within [-127, 127]; infinities are +-127, NaN is 0; all 0 for scale' = 0,
+ * and where a scale grows the codes of the block's earlier positions become the integers nearest to code * scale / scale'. Rows of a
+ * block behind the last position, and blocks not touched, are left as they were. A block that two sequences of one call write is the
+ * caller's mistake: it ends with codes and a scale of either (blocks that sequences share are full, and not written). */
+typedef struct HoloBlockCacheWriteCall {
+    HoloBufferRef k, v, starts, lengths, table, k_codes, k_scales, v_codes, v_scales;
+    uint32_t rows, sequences, kv_heads, dim, vdim, k_ld, v_ld, block_rows, blocks, table_ld;
+    uint8_t dtype;
+} HoloBlockCacheWriteCall;
+
+/* Extension. Row i of the n rows of sequence s sees positions j <= lengths[s] - n + i (it is its own last one, written before):
+ *   out = sum_j exp(scale q . k_j) v_j / sum_j exp(scale q . k_j)   over the values held, scores and sums f32
+ * q [rows, heads * dim] (pitch q_ld), output [rows, heads * vdim] (pitch ld), `dtype` f32, bf16 or f16 (rounded to nearest); dims up to
+ * 512; scale_bits as in PACKED_ATTENTION. A row that sees nothing is zero; rows of no sequence are left as they were. */
+typedef struct HoloBlockCacheAttentionCall {
+    HoloBufferRef q, starts, lengths, table, k_codes, k_scales, v_codes, v_scales, output;
+    uint32_t rows, sequences, heads, kv_heads, dim, vdim, q_ld, ld, block_rows, blocks, table_ld, scale_bits;
+    uint8_t dtype;
+} HoloBlockCacheAttentionCall;
+
+/* Extension. Rules on logits z [rows, vocab] (pitch ld, `dtype` f32, bf16 or f16) before a token is chosen, in f32, rounded once into
+ * output (pitch out_ld; it may be the logits themselves at the same pitch). Row r has the token history i32
+ * history[r, 0 .. spans[r].total), of which the first spans[r].prompt are the prompt (spans i32 [rows, 2] = prompt, total), and
+ * params f32 [rows, 4] = repetition, presence, frequency, temperature:
+ *   z = z > 0 ? z / repetition : z * repetition           for tokens anywhere in the history
+ *   z = z - (frequency * n + presence)                    for tokens that stand n >= 1 times behind the prompt
+ *   z = z + bias                                          for the tokens of bias_ids[bias_starts[r] .. bias_starts[r + 1])
+ *   z = z / temperature                                   where temperature > 0
+ *   z = -inf                                              where bit t % 32 of word t / 32 of the row's mask is 0
+ * bias_starts i32 [rows + 1], bias_ids i32 and bias_values f32 [biases]: a token named twice has the later value. masks u32
+ * [mask_rows, mask_ld]: row r is under mask mask_of[r] (i32 [rows]; -1: none; absent: mask r). history (with spans), params, the
+ * bias operands and masks may be absent. Ids outside the vocabulary are skipped; spans, starts and mask numbers outside their
+ * buffers are reported at the next synchronising call and count as empty. */
+typedef struct HoloLogitRulesCall {
+    HoloBufferRef logits, history, spans, params, bias_starts, bias_ids, bias_values, masks, mask_of, output;
+    uint32_t rows, vocab, ld, out_ld, history_ld, biases, mask_rows, mask_ld;
+    uint8_t dtype;
+} HoloLogitRulesCall;
+
 /* Extension. In-place sum over the context's tensor-parallel group (NCCL); a no-op when the
  * context has no group. */
 typedef struct HoloAllReduceCall {
@@ -609,6 +683,10 @@ typedef struct HoloKernelCall {
         HoloRetentionCall retention;
         HoloMoePlanCall moe_plan;
         HoloMoeCombineCall moe_combine;
+        HoloPackedAttentionCall packed_attention;
+        HoloBlockCacheWriteCall block_cache_write;
+        HoloBlockCacheAttentionCall block_cache_attention;
+        HoloLogitRulesCall logit_rules;
     } u;
 } HoloKernelCall;
 
