@@ -165,6 +165,9 @@ int32_t holo_launch_block_cache_write(holo_b200_ctx* ctx, const HoloBlockWriteAr
 }
 
 int32_t holo_launch_block_cache_attention(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a) {
+    bool taken;
+    HOLO_TRY(holo_try_block_attention(ctx, a, &taken));
+    if (taken) return HOLO_OK;
     CacheSource src = {a};
     return launch_general_rows(ctx, src, (uint64_t)a.c.rows * a.heads, a.c.vdim);
 }

@@ -52,6 +52,7 @@ struct holo_b200_ctx {
     uint32_t* dev_status = nullptr;
     float* causal_partials = nullptr;   // split-key partials of the causal attention, allocated once at a fixed size (graphs hold its address)
     float* latent_partials = nullptr;   // the same for the latent attention
+    float* block_partials = nullptr;    // partial results of the block cache's attention, allocated once at a fixed size
     float* split_partials = nullptr;    // split-key partials of the float-cache attention (HOLO_SPLIT_PARTIAL_BYTES, made with the context) or null
     bool session_capture = false;       // the stream is recording a session's own walk: its replays are ordered on this stream too
     uint32_t* attn_arrivals = nullptr;  // 65536 counters, zero between launches (decode attention)
@@ -426,6 +427,8 @@ struct HoloBlockAttnArgs {
     uint8_t dtype;
 };
 int32_t holo_launch_block_cache_attention(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a);
+// block_attention.cu: dims in steps of 16; *taken false: the shape is not one it serves
+int32_t holo_try_block_attention(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool* taken);
 // logit_rules.cu
 struct HoloLogitRulesArgs {
     const void* logits;
