@@ -67,10 +67,11 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool ta
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4u : 0u) : "memory");
 }
 
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
 // The list of planes: sequence by sequence, kv head by kv head, R rows by R rows; `at` counts the slabs of all planes before.
 struct Plane {
-    uint32_t seq, head, tile, tiles, first_row, n, slabs;
-    int64_t length, at;
+    uint32_t seq, head, tile, tiles, first_row, n, slabs, at;
+    int32_t length;
 };
 template <int R>
 __device__ __forceinline__ uint32_t rows_before(const Plane& p, uint32_t tile, uint32_t group) {       // positions up to the tile's last one
@@ -78,31 +79,23 @@ __device__ __forceinline__ uint32_t rows_before(const Plane& p, uint32_t tile, u
 }
 template <int R>
 __device__ __forceinline__ uint32_t slabs_of(const Plane& p, uint32_t tile, uint32_t group) {
-    const int64_t sees = p.length - p.n + rows_before<R>(p, tile, group);
-    return sees <= 0 ? 0u : (uint32_t)((sees + BA_SLAB - 1) / BA_SLAB);
+    const int32_t sees = p.length - (int32_t)(p.n - rows_before<R>(p, tile, group));
+    return sees <= 0 ? 0u : ((uint32_t)sees + BA_SLAB - 1) / BA_SLAB;
 }
 template <int R>
 __device__ __forceinline__ void read_sequence(const HoloBlockCache& c, uint32_t group, uint32_t s, Plane* p) {
-    int64_t b = s, e = (int64_t)s + 1;
+    int32_t b = (int32_t)s, e = (int32_t)s + 1;
     if (c.starts) {
         b = c.starts[s];
         e = c.starts[s + 1];
-        if (b < 0 || e < b || e > c.rows) b = e = 0;
+        if (b < 0 || e < b || e > (int32_t)c.rows) b = e = 0;
     }
     p->seq = s;
     p->first_row = (uint32_t)b;
     p->n = (uint32_t)(e - b);
-    p->length = min((int64_t)c.lengths[s], (int64_t)c.table_ld * c.block_rows);
-    p->tiles = (uint32_t)(((uint64_t)p->n * group + R - 1) / R);
+    p->length = max(0, min(c.lengths[s], (int32_t)(c.table_ld * c.block_rows)));
+    p->tiles = (p->n * group + R - 1) / R;
     p->head = p->tile = 0;
-}
-template <int R>
-__device__ __forceinline__ int64_t slabs_of_sequence(const HoloBlockCache& c, uint32_t group, uint32_t s) {
-    Plane p;
-    read_sequence<R>(c, group, s, &p);
-    int64_t sum = 0;
-    for (uint32_t t = 0; t < p.tiles; ++t) sum += slabs_of<R>(p, t, group);
-    return sum * c.kv_heads;
 }
 // On to the next plane that has slabs; slabs == 0: there is none.
 template <int R>
@@ -132,8 +125,6 @@ __global__ void __launch_bounds__(BA_THREADS, CTAS)
 block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
     constexpr int R = 4 * RT, KSTEPS = MAXD / 32, CHUNKS = MAXD / 16;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t s_sum[BA_WARPS];
-    __shared__ Plane s_first;
     __shared__ float s_row[R], s_ml[BA_WARPS][R][3];
     __shared__ uint32_t s_last;
     const HoloBlockAttnArgs& a = p.a;
@@ -146,63 +137,96 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
     holo_pdl_wait();
     if (blockIdx.x == 0) check_sequences(c.starts, c.lengths, c.sequences, c.rows, (int64_t)c.table_ld * br, c.status);
 
-    // ---- this CTA's share of the list ----
-    auto block_sum = [&](int64_t v, int64_t* before) {       // the sum over the block, and over the threads before this one
-        int64_t run = v;
+    // ---- this CTA's share of the list; every warp finds it by itself, four sequences a lane at a time ----
+    uint32_t cnt[4], upto = 0, sum = 0, all = 0;
+    auto count_chunk = [&](uint32_t s0) {
+        Plane seq[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t s = s0 + 4 * lane + i;
+            read_sequence<R>(c, group, min(s, c.sequences - 1), &seq[i]);
+            if (s >= c.sequences) seq[i].tiles = 0;
+        }
+        sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            cnt[i] = 0;
+#pragma unroll 1
+            for (uint32_t t = 0; t < seq[i].tiles; ++t) cnt[i] += slabs_of<R>(seq[i], t, group);
+            cnt[i] *= c.kv_heads;
+            sum += cnt[i];
+        }
+        upto = sum;
+#pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t u = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= (uint32_t)o) run += u;
+            const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= (uint32_t)o) upto += u;
         }
-        __syncthreads();
-        if (lane == 31) s_sum[warp] = run;
-        __syncthreads();
-        int64_t all = 0, base = 0;
-        for (int w = 0; w < BA_WARPS; ++w) {
-            if (w < (int)warp) base += s_sum[w];
-            all += s_sum[w];
-        }
-        *before = base + run - v;
-        return all;
+        all = __shfl_sync(0xffffffffu, upto, 31);
     };
-    int64_t total = 0, before = 0, mine = 0;
-    for (uint32_t s0 = 0; s0 < c.sequences; s0 += BA_THREADS) {
-        mine = s0 + tid < c.sequences ? slabs_of_sequence<R>(c, group, s0 + tid) : 0;
-        total += block_sum(mine, &before);
+    uint32_t total = 0;
+#pragma unroll 1
+    for (uint32_t s0 = 0; s0 < c.sequences; s0 += 128) {
+        count_chunk(s0);
+        total += all;
     }
     // a share is one slab a warp at least: fewer CTAs take part in a short list
-    const int64_t ctas = min((int64_t)gridDim.x, (total + BA_WARPS - 1) / BA_WARPS);
-    if ((int64_t)blockIdx.x >= ctas) return;
-    auto share = [&](int64_t cta) { return cta * total / ctas; };
-    const int64_t lo = share(blockIdx.x), hi = share((int64_t)blockIdx.x + 1);
+    const uint32_t ctas = min(gridDim.x, (total + BA_WARPS - 1) / BA_WARPS);
+    if (blockIdx.x >= ctas) return;
+    const uint32_t each = total / ctas, more_by_one = total - each * ctas;
+    auto share = [&](uint32_t cta) { return cta * each + min(cta, more_by_one); };
+    const uint32_t lo = share(blockIdx.x), hi = share(blockIdx.x + 1);
+    Plane first = {};
     {
-        int64_t run = 0;
-        for (uint32_t s0 = 0; s0 < c.sequences; s0 += BA_THREADS) {
-            int64_t all = total;
-            if (c.sequences > BA_THREADS) {
-                mine = s0 + tid < c.sequences ? slabs_of_sequence<R>(c, group, s0 + tid) : 0;
-                all = block_sum(mine, &before);
+        uint32_t run = 0, s0 = 0;
+        if (c.sequences > 128) {
+            for (;; s0 += 128) {
+                count_chunk(s0);
+                if (lo < run + all || s0 + 128 >= c.sequences) break;
+                run += all;
             }
-            if (lo < run + all) {
-                const int64_t at = run + before;
-                if (mine && lo >= at && lo < at + mine) {
-                    Plane f;
-                    read_sequence<R>(c, group, s0 + tid, &f);
-                    const int64_t each = mine / c.kv_heads;
-                    f.slabs = slabs_of<R>(f, 0, group);
-                    f.head = (uint32_t)((lo - at) / each);
-                    f.at = at + f.head * each;
-                    while (lo >= f.at + f.slabs && f.tile + 1 < f.tiles) {
-                        f.at += f.slabs;
-                        f.slabs = slabs_of<R>(f, ++f.tile, group);
-                    }
-                    s_first = f;
-                }
-                break;
-            }
-            run += all;
         }
-        __syncthreads();
+        uint32_t at = run + upto - sum, mine = 0, which = 0;
+        const uint32_t from = __ffs(__ballot_sync(0xffffffffu, lo < run + upto)) - 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (mine == 0) {
+                if (lo < at + cnt[i]) {
+                    mine = cnt[i];
+                    which = s0 + 4 * lane + i;
+                } else {
+                    at += cnt[i];
+                }
+            }
+        which = __shfl_sync(0xffffffffu, which, from);
+        at = __shfl_sync(0xffffffffu, at, from);
+        mine = __shfl_sync(0xffffffffu, mine, from);
+        read_sequence<R>(c, group, min(which, c.sequences - 1), &first);
+        const uint32_t a_head = max(mine / c.kv_heads, 1u);
+        first.head = min((lo - at) / a_head, c.kv_heads - 1);
+        first.at = at + first.head * a_head;
+        first.slabs = slabs_of<R>(first, 0, group);
+        while (lo >= first.at + first.slabs && first.tile + 1 < first.tiles) {
+            first.at += first.slabs;
+            first.slabs = slabs_of<R>(first, ++first.tile, group);
+        }
     }
+
+    // ---- a plane's rows: requested early, cut into digits when the plane begins ----
+    constexpr int OWN = R / BA_WARPS;
+    float x[OWN][MAXD / 32];
+    auto load_rows = [&](const Plane& f) {
+#pragma unroll
+        for (int y = 0; y < OWN; ++y) {
+            const uint32_t r = warp + BA_WARPS * y, flat = f.tile * R + r, i = flat / group, head = f.head * group + flat % group;
+#pragma unroll
+            for (int e = 0; e < MAXD / 32; ++e) {
+                const uint32_t d = lane + 32 * e;
+                x[y][e] = i < f.n && d < dim ? seq_load(a.q, (uint64_t)(f.first_row + i) * a.q_ld + (uint64_t)head * dim + d, a.dtype) : 0.0f;
+            }
+        }
+    };
+    load_rows(first);
 
     // ---- the ring of this warp ----
     const uint32_t ring = smem_u32(smem) + p.head_bytes + warp * STAGES * p.slab_bytes;
@@ -213,17 +237,23 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
     const bool one_block = br % BA_SLAB == 0;
     auto block_of = [&](uint32_t pos) { return p.br_shift >= 0 ? pos >> p.br_shift : pos / br; };
     auto ends_of = [&](const Plane& q, uint32_t* s0, uint32_t* s1) {      // the slabs of a plane that are this CTA's
-        *s0 = lo > q.at ? (uint32_t)(lo - q.at) : 0u;
-        *s1 = (uint32_t)min((int64_t)q.slabs, hi - q.at);
+        *s0 = lo > q.at ? lo - q.at : 0u;
+        *s1 = min(q.slabs, hi - q.at);
     };
-    Plane ahead = s_first;          // where the next slab to request lies
-    uint32_t ahead_slab, ahead_end, ahead_sees;
-    int ahead_id = -1;
+    Plane ahead = first;            // where the next slab to request lies
+    uint32_t ahead_slab, ahead_end, ahead_sees, ids_at = 0;
+    int ahead_id = -1, ids = -1;    // ids: with one block a slab, the blocks of this warp's next 32 slabs, a slab a lane
     bool more = true;
+    auto load_ids = [&]() {
+        const uint32_t slab = ahead_slab + BA_WARPS * lane;
+        ids_at = ahead_slab;
+        ids = slab < ahead_end ? c.table[(uint64_t)ahead.seq * c.table_ld + block_of(slab * BA_SLAB)] : -1;
+    };
     auto enter_ahead = [&]() {
         ends_of(ahead, &ahead_slab, &ahead_end);
         ahead_slab += warp;
-        ahead_sees = (uint32_t)(ahead.length - ahead.n + rows_before<R>(ahead, ahead.tile, group));
+        ahead_sees = (uint32_t)ahead.length - (ahead.n - rows_before<R>(ahead, ahead.tile, group));
+        if (one_block) load_ids();
     };
     auto find_ahead = [&]() {
         while (ahead_slab >= ahead_end) {
@@ -238,14 +268,18 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
             }
             enter_ahead();
         }
-        const uint32_t pos = ahead_slab * BA_SLAB + (one_block ? 0u : lane);
-        ahead_id = -1;
-        if (pos < ahead_sees) {
-            ahead_id = c.table[(uint64_t)ahead.seq * c.table_ld + block_of(pos)];
-            if ((uint32_t)ahead_id >= c.blocks) {
-                atomicOr(c.status, HOLO_STATUS_TABLE);
-                ahead_id = -1;
-            }
+        bool there = true;
+        if (one_block) {
+            if (ahead_slab - ids_at == BA_WARPS * 32) load_ids();
+            ahead_id = __shfl_sync(0xffffffffu, ids, (ahead_slab - ids_at) / BA_WARPS);
+        } else {
+            const uint32_t pos = ahead_slab * BA_SLAB + lane;
+            there = pos < ahead_sees;
+            ahead_id = there ? c.table[(uint64_t)ahead.seq * c.table_ld + block_of(pos)] : -1;
+        }
+        if ((uint32_t)ahead_id >= c.blocks) {
+            if (there) atomicOr(c.status, HOLO_STATUS_TABLE);
+            ahead_id = -1;
         }
     };
     auto request = [&](uint32_t stage) {
@@ -296,34 +330,36 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
     };
     enter_ahead();
     find_ahead();
-#pragma unroll
-    for (int s = 0; s < STAGES; ++s) request(s);
+#pragma unroll 1
+    for (int s = 0; s < STAGES - 1; ++s) request(s);
 
     uint32_t stage = 0;
-    Plane at = s_first;
+    Plane at = first;
+#pragma unroll 1
     for (;;) {
         // ---- one plane: its rows' digits, then the slabs of it that are this CTA's ----
         const uint32_t rows = min((uint32_t)R, at.n * group - at.tile * R);
-        for (uint32_t r = warp; r < R; r += BA_WARPS) {
-            const uint32_t flat = at.tile * R + r, i = flat / group, head = at.head * group + flat % group;
-            float x[MAXD / 32], most = 0.0f;
+#pragma unroll
+        for (int y = 0; y < OWN; ++y) {
+            const uint32_t r = warp + BA_WARPS * y;
+            float most = 0.0f;
             bool finite = true;
 #pragma unroll
             for (int e = 0; e < MAXD / 32; ++e) {
-                const uint32_t d = lane + 32 * e;
-                x[e] = r < rows && d < dim ? seq_load(a.q, (uint64_t)(at.first_row + i) * a.q_ld + (uint64_t)head * dim + d, a.dtype) : 0.0f;
-                most = fmaxf(most, fabsf(x[e]));
-                finite = finite && fabsf(x[e]) < INFINITY;
+                most = fmaxf(most, fabsf(x[y][e]));
+                finite = finite && fabsf(x[y][e]) < INFINITY;
             }
-            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            // magnitudes order as their bits do
+            most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
             finite = __all_sync(0xffffffffu, finite);
             // 2^e <= most < 2^(e + 1); two factors, since 2^(29 - e) alone may overflow
-            const int up = finite && most > 0.0f ? 29 - ilogbf(most) : 0;
-            const float f0 = exp2f((float)(up / 2)), f1 = exp2f((float)(up - up / 2));
+            const uint32_t bits = __float_as_uint(most);
+            const int up = finite && bits ? 29 - (bits >> 23 ? (int)(bits >> 23) - 127 : -118 - __clz((int)bits)) : 0;
+            const float f0 = power_of_two(up / 2), f1 = power_of_two(up - up / 2);
             uint8_t* to = smem + (r >> 2) * 16 * MAXD + (r & 3u) * MAXD + lane;       // digit g of row r is row 4 g + r % 4 of product r / 4
 #pragma unroll
             for (int e = 0; e < MAXD / 32; ++e) {
-                int v = finite ? __float2int_rn(x[e] * f0 * f1) : 0;
+                int v = finite ? __float2int_rn(x[y][e] * f0 * f1) : 0;
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const int digit = (int)(int8_t)v;
@@ -331,7 +367,7 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
                     v = (v - digit) >> 8;
                 }
             }
-            if (lane == 0) s_row[r] = finite ? a.scale * LOG2E * exp2f((float)(-(up / 2))) * exp2f((float)(-(up - up / 2))) : NAN;
+            if (lane == 0) s_row[r] = finite ? a.scale * LOG2E * power_of_two(-(up / 2)) * power_of_two(-(up - up / 2)) : NAN;
         }
         __syncthreads();
         uint32_t q[RT][KSTEPS][4];
@@ -344,8 +380,8 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
         // this lane's row (four rows: in both halves of the warp)
         const uint32_t row = RT == 1 ? quad & 3u : quad, row_at = (at.tile * R + min(row, rows - 1)) / group;
         const float row_scale = s_row[row];
-        const uint32_t limit = (uint32_t)max((int64_t)0, at.length - at.n + row_at + 1);
-        const uint32_t common = (uint32_t)max((int64_t)0, at.length - at.n + (at.tile * R) / group + 1);      // keys that all rows see
+        const uint32_t limit = (uint32_t)max(0, at.length - (int32_t)(at.n - row_at - 1));
+        const uint32_t common = (uint32_t)max(0, at.length - (int32_t)(at.n - (at.tile * R) / group - 1));      // keys that all rows see
         float o[CHUNKS][4], top = -INFINITY, sum = 0.0f;
         int lift = -1000;           // the exponent that value scales are relative to
 #pragma unroll
@@ -356,6 +392,7 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
         ends_of(at, &from, &to);
 #pragma unroll 1
         for (uint32_t slab = from + warp; slab < to; slab += BA_WARPS) {
+            request(stage == 0 ? STAGES - 1 : stage - 1);      // where the slab before this one was
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
             __syncwarp();
             const uint32_t k_at = ring + stage * p.slab_bytes + lane * k_pitch, v_at = ring + stage * p.slab_bytes + BA_SLAB * k_pitch + lane * v_pitch;
@@ -418,7 +455,7 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
             else e = __reduce_max_sync(0xffffffffu, e);
             if (__any_sync(0xffffffffu, most > top) || e > lift) {
                 const int higher = max(e, lift);
-                const float turn = lift == -1000 ? 0.0f : exp2f((float)max(lift - higher, -250));
+                const float turn = lift == -1000 ? 0.0f : lift - higher < -126 ? 0.0f : power_of_two(lift - higher);
                 lift = higher;
                 const float t = fmaxf(top, most), f = top == t ? 1.0f : ex2(top - t);
                 top = t;
@@ -431,7 +468,7 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
                     o[i][2] *= g0; o[i][3] *= g1;
                 }
             }
-            const float least = top == -INFINITY ? 0.0f : top, raise = __uint_as_float((uint32_t)(14 - lift + 127) << 23);
+            const float least = top == -INFINITY ? 0.0f : top, raise = power_of_two(min(14 - lift, 127));
             uint32_t w[4], w2[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -461,7 +498,6 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
                 }
             }
             __syncwarp();       // the slab has been read
-            request(stage);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
         // ---- the four warps' results, through the memory of the digits ----
@@ -470,9 +506,14 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
         if (in_quad == 0 && (RT == 2 || lane < 16)) {
             s_ml[warp][row][0] = top;
             s_ml[warp][row][1] = sum;
-            s_ml[warp][row][2] = lift == -1000 ? 0.0f : exp2f((float)(lift - 14));
+            s_ml[warp][row][2] = lift == -1000 ? 0.0f : power_of_two(lift - 14);
         }
+        Plane next = at;
         const bool begins = at.at >= lo, ends = at.at + at.slabs <= hi, whole = begins && ends;
+        if (at.at + at.slabs < hi) {
+            next_plane<R>(c, group, &next);
+            if (next.slabs) load_rows(next);
+        }
         float* partial = p.partials + ((uint64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * R * (vdim + 2);
         float* s_o = reinterpret_cast<float*>(smem);       // [warp][R][vdim]
         const uint32_t columns = vdim / 4;
@@ -530,50 +571,69 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
         }
         if (!whole) {
             // the CTAs that share the plane, and its counter: that of the CTA it begins in
-            auto owner = [&](int64_t slab) {
-                int64_t w = slab * ctas / total;
-                while (share(w) > slab) --w;
-                while (share(w + 1) <= slab) ++w;
-                return w;
+            auto owner = [&](uint32_t slab) {
+                const uint32_t longer = more_by_one * (each + 1);
+                return slab < longer ? slab / (each + 1) : more_by_one + (slab - longer) / each;
             };
-            const int64_t first = owner(at.at), last = owner(at.at + at.slabs - 1);
+            const uint32_t from_cta = owner(at.at), to_cta = owner(at.at + at.slabs - 1), count = to_cta - from_cta + 1;
             __syncthreads();
             if (tid == 0) {
-                __threadfence();
-                const uint32_t n = atomicAdd(p.arrivals + first, 1u) + 1;
-                s_last = n == (uint32_t)(last - first + 1);
-                if (s_last) p.arrivals[first] = 0;
-                __threadfence();
+                uint32_t n;
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(n) : "l"(p.arrivals + from_cta) : "memory");
+                s_last = n + 1 == count;
+                if (s_last) p.arrivals[from_cta] = 0;
             }
             __syncthreads();
             if (s_last) {
-                const float* base = p.partials + (uint64_t)first * 2 * R * (vdim + 2);
-                const uint32_t count = (uint32_t)(last - first + 1), step = 2 * R * (vdim + 2), own = R * (vdim + 2);
+                const float* base = p.partials + (uint64_t)from_cta * 2 * R * (vdim + 2);
+                const uint32_t step = 2 * R * (vdim + 2), own = R * (vdim + 2);
+                auto part = [&](uint32_t w, uint32_t r) { return base + (uint64_t)w * step + (w == 0 ? own : 0u) + r * (vdim + 2); };
+                // the parts' weights first: a warp a row, a part a lane; then a column of all parts at a time
+                float* s_f = s_o;         // [R][count]
+#pragma unroll 1
+                for (uint32_t r = warp; r < rows; r += BA_WARPS) {
+                    float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
+                    for (uint32_t w = lane; w < count; w += 64) {
+                        const float2 y0 = __ldcg(reinterpret_cast<const float2*>(part(w, r) + vdim));
+                        const float2 y1 = w + 32 < count ? __ldcg(reinterpret_cast<const float2*>(part(w + 32, r) + vdim)) : make_float2(-INFINITY, 0.0f);
+                        const float t = fmaxf(m, fmaxf(y0.x, y1.x));
+                        s_f[r * count + w] = y0.x;
+                        if (w + 32 < count) s_f[r * count + w + 32] = y1.x;
+                        // parts that saw nothing have no sum; NaN is not 0
+                        if (l != 0.0f) l *= ex2(m - t);
+                        if (y0.y != 0.0f) l = fmaf(ex2(y0.x - t), y0.y, l);
+                        if (y1.y != 0.0f) l = fmaf(ex2(y1.x - t), y1.y, l);
+                        m = t;
+                    }
+                    float top_m = m;
+                    for (int o = 16; o > 0; o >>= 1) top_m = fmaxf(top_m, __shfl_xor_sync(0xffffffffu, top_m, o));
+                    if (l != 0.0f) l *= ex2(m - top_m);
+                    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+                    __syncwarp();
+                    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+                    for (uint32_t w = lane; w < count; w += 32) {
+                        const float x0 = s_f[r * count + w];
+                        s_f[r * count + w] = l == 0.0f || (x0 == -INFINITY && l == l) ? 0.0f : ex2(x0 - top_m) * inv;
+                    }
+                }
+                __syncthreads();
                 for (uint32_t i = tid; i < rows * columns; i += BA_THREADS) {
                     const uint32_t r = i / columns, col = 4 * (i % columns);
-                    const float* of = base + r * (vdim + 2);
-                    float m = -INFINITY, l = 0.0f;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
+#pragma unroll 16
                     for (uint32_t w = 0; w < count; ++w) {
-                        const float* from2 = of + (uint64_t)w * step + (w == 0 ? own : 0u);
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(from2 + vdim)), y0 = __ldcg(reinterpret_cast<const float2*>(from2 + col)),
-                                     y1 = __ldcg(reinterpret_cast<const float2*>(from2 + col + 2));
-                        if (ml.y != 0.0f) {
-                            const float t = fmaxf(m, ml.x), f = m == t ? 1.0f : ex2(m - t), g = ex2(ml.x - t);
-                            m = t;
-                            l = fmaf(g, ml.y, l * f);
-                            v = make_float4(fmaf(g, y0.x, v.x * f), fmaf(g, y0.y, v.y * f), fmaf(g, y1.x, v.z * f), fmaf(g, y1.y, v.w * f));
-                        }
+                        const float* of = part(w, r) + col;
+                        const float2 y0 = __ldcg(reinterpret_cast<const float2*>(of)), y1 = __ldcg(reinterpret_cast<const float2*>(of + 2));
+                        const float f = s_f[r * count + w];
+                        v = make_float4(fmaf(f, y0.x, v.x), fmaf(f, y0.y, v.y), fmaf(f, y1.x, v.z), fmaf(f, y1.y, v.w));
                     }
-                    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-                    store4(r, col, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                    store4(r, col, v);
                 }
             }
         }
-        if (at.at + at.slabs >= hi) break;
-        next_plane<R>(c, group, &at);
-        if (!at.slabs) break;
+        if (at.at + at.slabs >= hi || !next.slabs) break;
+        at = next;
         __syncthreads();        // the results have been read: the next plane's digits may come
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -590,7 +650,10 @@ int32_t launch_block_attention(holo_b200_ctx* ctx, BlockAttnParams& p) {
     p.v_pitch = pitch(vdim);
     p.slab_bytes = BA_SLAB * (p.k_pitch + p.v_pitch) + 256;
     const uint32_t digits = RT * 16 * MAXD, merge = BA_WARPS * 4 * RT * vdim * 4;
-    p.head_bytes = ((digits > merge ? digits : merge) + 127u) & ~127u;
+    const uint32_t ctas = (uint32_t)ctx->sm_count * CTAS < BA_MOST_CTAS ? (uint32_t)ctx->sm_count * CTAS : BA_MOST_CTAS;
+    p.head_bytes = digits > merge ? digits : merge;
+    if (p.head_bytes < 16 * RT * ctas) p.head_bytes = 16 * RT * ctas;      // the weights of a plane's parts
+    p.head_bytes = (p.head_bytes + 127u) & ~127u;
     const uint32_t smem = p.head_bytes + BA_WARPS * STAGES * p.slab_bytes;
     static thread_local int configured_device = -1;
     static thread_local uint32_t configured = 0;
@@ -599,8 +662,7 @@ int32_t launch_block_attention(holo_b200_ctx* ctx, BlockAttnParams& p) {
         configured_device = ctx->device;
         configured = smem;
     }
-    const uint32_t ctas = (uint32_t)ctx->sm_count * CTAS;
-    HOLO_CUDA(holo_launch_kernel(ctx, block_attention_kernel<RT, MAXD, EXACT, SECOND, STAGES, CTAS>, dim3(ctas < BA_MOST_CTAS ? ctas : BA_MOST_CTAS), dim3(BA_THREADS), smem, 1, p));
+    HOLO_CUDA(holo_launch_kernel(ctx, block_attention_kernel<RT, MAXD, EXACT, SECOND, STAGES, CTAS>, dim3(ctas), dim3(BA_THREADS), smem, 1, p));
     ctx->launches++;
     return HOLO_OK;
 }
@@ -609,7 +671,7 @@ int32_t launch_block_attention_dims(holo_b200_ctx* ctx, BlockAttnParams& p) {
     const HoloBlockCache& c = p.a.c;
     const uint32_t d = c.dim > c.vdim ? c.dim : c.vdim;
     const bool exact = c.dim == c.vdim && (d == 64 || d == 128);
-    if (d <= 64) return exact ? launch_block_attention<RT, 64, true, SECOND, 3, 3>(ctx, p) : launch_block_attention<RT, 64, false, SECOND, 3, 3>(ctx, p);
+    if (d <= 64) return exact ? launch_block_attention<RT, 64, true, SECOND, 4, 2>(ctx, p) : launch_block_attention<RT, 64, false, SECOND, 4, 2>(ctx, p);
     if (d <= 128) return exact ? launch_block_attention<RT, 128, true, SECOND, 3, 2>(ctx, p) : launch_block_attention<RT, 128, false, SECOND, 3, 2>(ctx, p);
     return launch_block_attention<RT, 256, false, SECOND, 2, 1>(ctx, p);
 }
@@ -621,7 +683,10 @@ int32_t holo_try_block_attention(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a,
     const HoloBlockCache& c = a.c;
     if (c.dim % 16 != 0 || c.vdim % 16 != 0 || c.dim > 256 || c.vdim > 256) return HOLO_OK;
     if ((((uintptr_t)c.k_codes | (uintptr_t)c.v_codes) & 15u) != 0) return HOLO_OK;
-    if ((uint64_t)c.blocks * c.kv_heads * c.block_rows >= 0xffffffffull || (uint64_t)c.rows * a.heads > 0x7fffffffull) return HOLO_OK;      // row numbers of 32 bits
+    // row numbers, and slabs of the whole list, of 32 bits
+    const uint64_t tiles = ((uint64_t)c.rows * (a.heads / c.kv_heads) / 4 + c.sequences) * c.kv_heads;
+    if ((uint64_t)c.blocks * c.kv_heads * c.block_rows >= 0xffffffffull || (uint64_t)c.rows * a.heads > 0x7fffffffull) return HOLO_OK;
+    if (tiles > 0x7fffffffull / (((uint64_t)c.table_ld * c.block_rows + BA_SLAB - 1) / BA_SLAB)) return HOLO_OK;
     if (!ctx->block_partials) {
         cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
         HOLO_CUDA(cudaStreamIsCapturing(ctx->stream, &capturing));
