@@ -138,7 +138,8 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
     if (blockIdx.x == 0) check_sequences(c.starts, c.lengths, c.sequences, c.rows, (int64_t)c.table_ld * br, c.status);
 
     // ---- this CTA's share of the list; every warp finds it by itself, four sequences a lane at a time ----
-    uint32_t cnt[4], upto = 0, sum = 0, all = 0;
+    uint32_t cnt[4], upto = 0, sum = 0, all = 0, planes = 0;
+    uint32_t unit = 1;              // slabs of a piece: 1, or where no CTA takes pieces of two planes, its share
     auto count_chunk = [&](uint32_t s0) {
         Plane seq[4];
 #pragma unroll
@@ -152,9 +153,10 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
         for (int i = 0; i < 4; ++i) {
             cnt[i] = 0;
 #pragma unroll 1
-            for (uint32_t t = 0; t < seq[i].tiles; ++t) cnt[i] += slabs_of<R>(seq[i], t, group);
+            for (uint32_t t = 0; t < seq[i].tiles; ++t) cnt[i] += (slabs_of<R>(seq[i], t, group) + unit - 1) / unit;
             cnt[i] *= c.kv_heads;
             sum += cnt[i];
+            planes += seq[i].tiles;
         }
         upto = sum;
 #pragma unroll
@@ -170,28 +172,40 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
         count_chunk(s0);
         total += all;
     }
-    // a share is one slab a warp at least: fewer CTAs take part in a short list
-    const uint32_t ctas = min(gridDim.x, (total + BA_WARPS - 1) / BA_WARPS);
-    if (blockIdx.x >= ctas) return;
-    const uint32_t each = total / ctas, more_by_one = total - each * ctas;
-    auto share = [&](uint32_t cta) { return cta * each + min(cta, more_by_one); };
-    const uint32_t lo = share(blockIdx.x), hi = share(blockIdx.x + 1);
+    planes = __reduce_add_sync(0xffffffffu, planes) * c.kv_heads;
+    // A share is one slab a warp at least: fewer CTAs take part in a short list. Few planes are cut into pieces of their own, at most as
+    // many as there are CTAs, where that lengthens a share by less than the 8 slabs (2 a warp) that a second plane costs a CTA.
+    const uint32_t grid = gridDim.x;
+    const bool apart = planes < grid && (uint64_t)total * planes <= 8ull * grid * (grid - planes);
+    uint32_t ctas = min(grid, (total + BA_WARPS - 1) / BA_WARPS), each = 0, more_by_one = 0, want = 0;
+    if (apart) {
+        unit = max((total + grid - planes - 1) / (grid - planes), (uint32_t)BA_WARPS);
+        want = blockIdx.x;
+    } else {
+        if (blockIdx.x >= ctas) return;
+        each = total / ctas;
+        more_by_one = total - each * ctas;
+        want = blockIdx.x * each + min(blockIdx.x, more_by_one);
+    }
     Plane first = {};
+    uint32_t lo, hi, part = 0;      // this CTA's slabs; apart: of its plane, of which they are the part of this number
     {
         uint32_t run = 0, s0 = 0;
-        if (c.sequences > 128) {
-            for (;; s0 += 128) {
-                count_chunk(s0);
-                if (lo < run + all || s0 + 128 >= c.sequences) break;
-                run += all;
-            }
+        bool found = false;
+#pragma unroll 1
+        for (;; s0 += 128) {
+            if (apart || c.sequences > 128) count_chunk(s0);
+            found = want < run + all;
+            if (found || s0 + 128 >= c.sequences) break;
+            run += all;
         }
+        if (!found) return;
         uint32_t at = run + upto - sum, mine = 0, which = 0;
-        const uint32_t from = __ffs(__ballot_sync(0xffffffffu, lo < run + upto)) - 1;
+        const uint32_t from = __ffs(__ballot_sync(0xffffffffu, want < run + upto)) - 1;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (mine == 0) {
-                if (lo < at + cnt[i]) {
+                if (want < at + cnt[i]) {
                     mine = cnt[i];
                     which = s0 + 4 * lane + i;
                 } else {
@@ -203,12 +217,23 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
         mine = __shfl_sync(0xffffffffu, mine, from);
         read_sequence<R>(c, group, min(which, c.sequences - 1), &first);
         const uint32_t a_head = max(mine / c.kv_heads, 1u);
-        first.head = min((lo - at) / a_head, c.kv_heads - 1);
+        first.head = min((want - at) / a_head, c.kv_heads - 1);
         first.at = at + first.head * a_head;
         first.slabs = slabs_of<R>(first, 0, group);
-        while (lo >= first.at + first.slabs && first.tile + 1 < first.tiles) {
-            first.at += first.slabs;
+        for (;;) {
+            const uint32_t pieces = (first.slabs + unit - 1) / unit;
+            if (want < first.at + pieces || first.tile + 1 >= first.tiles) break;
+            first.at += pieces;
             first.slabs = slabs_of<R>(first, ++first.tile, group);
+        }
+        if (apart) {
+            part = want - first.at;
+            first.at = 0;
+            lo = part * unit;
+            hi = min(lo + unit, first.slabs);
+        } else {
+            lo = want;
+            hi = (blockIdx.x + 1) * each + min(blockIdx.x + 1, more_by_one);
         }
     }
 
@@ -242,18 +267,17 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
     };
     Plane ahead = first;            // where the next slab to request lies
     uint32_t ahead_slab, ahead_end, ahead_sees, ids_at = 0;
-    int ahead_id = -1, ids = -1;    // ids: with one block a slab, the blocks of this warp's next 32 slabs, a slab a lane
+    int ahead_id = -1, ids = -1;    // ids: the blocks from number ids_at on, one a lane
     bool more = true;
-    auto load_ids = [&]() {
-        const uint32_t slab = ahead_slab + BA_WARPS * lane;
-        ids_at = ahead_slab;
-        ids = slab < ahead_end ? c.table[(uint64_t)ahead.seq * c.table_ld + block_of(slab * BA_SLAB)] : -1;
+    auto load_ids = [&](uint32_t blk) {
+        ids_at = blk;
+        ids = blk + lane <= block_of(ahead_sees - 1) ? c.table[(uint64_t)ahead.seq * c.table_ld + blk + lane] : -1;
     };
     auto enter_ahead = [&]() {
         ends_of(ahead, &ahead_slab, &ahead_end);
         ahead_slab += warp;
         ahead_sees = (uint32_t)ahead.length - (ahead.n - rows_before<R>(ahead, ahead.tile, group));
-        if (one_block) load_ids();
+        load_ids(block_of(ahead_slab * BA_SLAB));
     };
     auto find_ahead = [&]() {
         while (ahead_slab >= ahead_end) {
@@ -268,15 +292,11 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
             }
             enter_ahead();
         }
-        bool there = true;
-        if (one_block) {
-            if (ahead_slab - ids_at == BA_WARPS * 32) load_ids();
-            ahead_id = __shfl_sync(0xffffffffu, ids, (ahead_slab - ids_at) / BA_WARPS);
-        } else {
-            const uint32_t pos = ahead_slab * BA_SLAB + lane;
-            there = pos < ahead_sees;
-            ahead_id = there ? c.table[(uint64_t)ahead.seq * c.table_ld + block_of(pos)] : -1;
-        }
+        const uint32_t at_pos = ahead_slab * BA_SLAB, pos = at_pos + (one_block ? 0u : lane);
+        if (block_of(min(at_pos + BA_SLAB, ahead_sees) - 1) - ids_at > 31) load_ids(block_of(at_pos));
+        const bool there = pos < ahead_sees;
+        ahead_id = __shfl_sync(0xffffffffu, ids, there ? block_of(pos) - ids_at : 0u);
+        if (!there) ahead_id = -1;
         if ((uint32_t)ahead_id >= c.blocks) {
             if (there) atomicOr(c.status, HOLO_STATUS_TABLE);
             ahead_id = -1;
@@ -575,7 +595,8 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
                 const uint32_t longer = more_by_one * (each + 1);
                 return slab < longer ? slab / (each + 1) : more_by_one + (slab - longer) / each;
             };
-            const uint32_t from_cta = owner(at.at), to_cta = owner(at.at + at.slabs - 1), count = to_cta - from_cta + 1;
+            const uint32_t from_cta = apart ? blockIdx.x - part : owner(at.at);
+            const uint32_t count = apart ? (at.slabs + unit - 1) / unit : owner(at.at + at.slabs - 1) - from_cta + 1;
             __syncthreads();
             if (tid == 0) {
                 uint32_t n;
