@@ -36,6 +36,9 @@ struct PackedSource {
 }  // namespace
 
 int32_t holo_launch_packed_attention(holo_b200_ctx* ctx, const HoloPackedArgs& a) {
+    bool taken;
+    HOLO_TRY(holo_try_packed_tile(ctx, a, &taken));
+    if (taken) return HOLO_OK;
     PackedSource src = {a};
     return launch_general_rows(ctx, src, (uint64_t)a.rows * a.heads, a.vdim);
 }
