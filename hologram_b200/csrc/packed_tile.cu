@@ -5,8 +5,9 @@
 // tiles. A CTA takes one or two neighbouring query tiles of a head after another (persistent: the next tiles' loads and scores run
 // while the last ones are stored):
 //   warp 0     TMA producer: the query tiles, K and V tiles through rings of two
-//   warp 1     tcgen05.mma issuer: S = Q K^T, then O += P V with P read from TMEM, the two query tiles in turn
-//   warps 2-9  softmax, one group of four warps per query tile, one thread per row: running maximum, exponentials, row sum;
+//   warps 1, 2 tcgen05.mma issuers, one for each query tile: S = Q K^T, then O += P V with P read from TMEM. A wait or a commit costs an
+//              issuer 150 to 300 cycles while the tensor core has the shared memory; two of them hide each other's (8192 rows: 353 -> 0 us)
+//   warps 4-11 softmax, one group of four warps per query tile, one thread per row: running maximum, exponentials, row sum;
 //              a row's O is rescaled in TMEM only when its maximum grows by more than 2^GROWTH
 // The weights are rounded to the operands' type (2^-9 of a weight in bf16, 2^-12 in f16, at most), sums stay f32: a rounded weight moves
 // a result by as much as the result's own rounding does, and a second term for the remainder would be half as many products again.
@@ -20,7 +21,8 @@
 
 namespace {
 
-constexpr int PT_WARPS = 10;
+constexpr int PT_WARPS = 12;
+constexpr uint32_t PT_ITEMS = 128;       // items of a CTA that are worked out beforehand
 constexpr float PT_GROWTH = 8.0f;
 constexpr uint32_t PT_STARTS = 4096;      // starts kept in shared memory; more are read where they are
 
@@ -37,6 +39,33 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 }
 template <bool F16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) { return F16 ? pack_half(lo, hi) : pack_bf16(lo, hi); }
+
+// The issuer runs with all its lanes and one of them is elected by a predicate, never by a branch: descriptors then stay in uniform registers,
+// where the instruction wants them. Behind a branch each product cost the thread 100 cycles, half as much again as the tensor core.
+__device__ __forceinline__ void elected_ss(uint32_t elected, uint32_t tmem_d, uint32_t a, uint32_t a_high, uint32_t b, uint32_t b_high, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred p, e;\n.reg .b64 x, y;\nmov.b64 x, {%1, %2};\nmov.b64 y, {%3, %4};\nsetp.ne.b32 e, %7, 0;\nsetp.ne.b32 p, %6, 0;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, p;\n}\n"
+        ::"r"(tmem_d), "r"(a), "r"(a_high), "r"(b), "r"(b_high), "r"(idesc), "r"(accumulate), "r"(elected)
+        : "memory");
+}
+__device__ __forceinline__ void elected_ts(uint32_t elected, uint32_t tmem_d, uint32_t tmem_a, uint32_t b, uint32_t b_high, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred p, e;\n.reg .b64 y;\nmov.b64 y, {%2, %3};\nsetp.ne.b32 e, %6, 0;\nsetp.ne.b32 p, %5, 0;\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n}\n"
+        ::"r"(tmem_d), "r"(tmem_a), "r"(b), "r"(b_high), "r"(idesc), "r"(accumulate), "r"(elected)
+        : "memory");
+}
+__device__ __forceinline__ void elected_commit(uint32_t elected, uint32_t bar) {
+    asm volatile("{\n.reg .pred e;\nsetp.ne.b32 e, %1, 0;\n@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar), "r"(elected) : "memory");
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// An item: the query tiles of a pair (the last ones first: in a long causal sequence they have the most keys) and a head. Tile q walks the
+// key tiles [from[q], to[q]) of 128 keys each, counted from `anchor`; left[q]: keys from there to its last one.
+struct PackedItem {
+    uint32_t row0, head, anchor, tiles, from[2], to[2], left[2];
+};
 
 // Keys that some row of a query tile sees, [begin, end); the same for every thread that asks.
 struct KeyRange {
@@ -128,7 +157,8 @@ __device__ __forceinline__ bool pt_wait(uint32_t bar, uint32_t parity, volatile 
 
 constexpr float PT_WILD = 0x1p22f;     // from here on a fused exponent of the largest score is off by whole units
 
-template <bool F16>
+// KS: dim / 16 where that is 4 or 8, else 0
+template <bool F16, int KS>
 __global__ void __launch_bounds__(PT_WARPS * 32, 1)
 packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                    const __grid_constant__ PackedTileParams p) {
@@ -144,16 +174,18 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                    bar_s = bars + 80, bar_pa = bars + 96, bar_pb = bars + 112, bar_pv = bars + 128;
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sm + (bars - base) + 160);
     volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(sm + (bars - base) + 164);
-    int32_t* s_starts = reinterpret_cast<int32_t*>(sm + (bars - base) + 256);
+    PackedItem* s_items = reinterpret_cast<PackedItem*>(sm + (bars - base) + 256);
+    int32_t* s_starts = reinterpret_cast<int32_t*>(sm + (bars - base) + 256 + PT_ITEMS * sizeof(PackedItem));
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(bar_q_full, 1);
-        mbar_init(bar_q_empty, 1);
+        mbar_init(bar_q_empty, p.nq);         // one arrival per issuer
+
         for (int s = 0; s < 2; ++s) {
             mbar_init(bar_k_full + 8 * s, 1);
-            mbar_init(bar_k_empty + 8 * s, 1);
+            mbar_init(bar_k_empty + 8 * s, p.nq);
             mbar_init(bar_v_full + 8 * s, 1);
-            mbar_init(bar_v_empty + 8 * s, 1);
+            mbar_init(bar_v_empty + 8 * s, p.nq);
             mbar_init(bar_s + 8 * s, 1);
             mbar_init(bar_pa + 8 * s, 4);     // one arrival per softmax warp
             mbar_init(bar_pb + 8 * s, 4);
@@ -178,13 +210,8 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const uint32_t tmem_base = *s_tmem;
     const int32_t* starts = kept ? s_starts : a.starts;
 
-    // An item: the query tiles of a pair (the last ones first: in a long causal sequence they have the most keys) and a head. Tile q walks
-    // the key tiles [from[q], to[q]) of 128 keys each, counted from `anchor`.
-    struct Item {
-        uint32_t row0, head, anchor, from[2], to[2], end[2], tiles;
-    };
-    auto item_of = [&](uint32_t i) {
-        Item it;
+    auto make_item = [&](uint32_t i) {
+        PackedItem it;
         it.head = i % a.heads;
         it.row0 = (p.pairs - 1 - i / a.heads) * p.nq * 128;
         KeyRange r[2];
@@ -197,10 +224,17 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             const bool any = r[q].end > r[q].begin && r[q].begin >= it.anchor;
             it.from[q] = any ? (r[q].begin - it.anchor) / 128 : 0u;
             it.to[q] = any ? (r[q].end - it.anchor + 127) / 128 : 0u;
-            it.end[q] = r[q].end;
+            it.left[q] = r[q].end - it.anchor;
             it.tiles = max(it.tiles, it.to[q]);
         }
         return it;
+    };
+    // a thread an item
+    if (threadIdx.x < PT_ITEMS && blockIdx.x + threadIdx.x * gridDim.x < p.items) s_items[threadIdx.x] = make_item(blockIdx.x + threadIdx.x * gridDim.x);
+    __syncthreads();
+    auto item_of = [&](uint32_t i) {
+        const uint32_t n = (i - blockIdx.x) / gridDim.x;
+        return n < PT_ITEMS ? s_items[n] : make_item(i);
     };
 
     if (warp == 0) {
@@ -209,7 +243,7 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             uint32_t nq = 0, nk = 0, nv = 0;       // copies of each kind so far
             bool ok = true;
             for (uint32_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-                const Item it = item_of(i);
+                const PackedItem it = item_of(i);
                 if (it.tiles == 0) continue;
                 const int g = (int)(it.head / (a.heads / a.kv_heads));
                 ok = nq == 0 || pt_wait(bar_q_empty, (nq - 1) & 1u, s_abort, a.status);
@@ -243,87 +277,86 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                     for (uint32_t x = 0; x < WAIT_LIMIT && !mbar_try_wait(bar_v_full + 8 * (t & 1), (t >> 1) & 1); ++x) __nanosleep(64);
             }
         }
-    } else if (warp == 1) {
-        // ---------------- MMA issuer ----------------
-        if (lane == 0) {
+    } else if (warp <= 2) {
+        // ---------------- MMA issuers ----------------
+        if (warp <= p.nq) {
+            const uint32_t q = uniform(warp - 1), elected = lane == 0;
             // D = f32, A and B of the call's type, M = 128; S: both operands K-major, N = 128; O: V is N-major, N = vdim
             const uint32_t type = F16 ? 0u : (1u << 7) | (1u << 10);
             const uint32_t idesc_s = (1u << 4) | type | ((128u >> 3) << 17) | ((128u >> 4) << 24);
             const uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((a.vdim >> 3) << 17) | ((128u >> 4) << 24);
-            const uint64_t first_q = smem_desc(s_q, 16, 1024), first_v = smem_desc(s_v, TILE_CHUNK, 1024);
-            const uint32_t desc_q = (uint32_t)first_q, desc_k = (uint32_t)smem_desc(s_k, 16, 1024), high_s = (uint32_t)(first_q >> 32);
-            const uint32_t desc_v = (uint32_t)first_v, high_v = (uint32_t)(first_v >> 32);
-            const uint32_t ksteps = a.dim / 16;
-            uint32_t nq = 0, nk = 0, nv = 0, np[2] = {0, 0};
+            const uint64_t first_q = smem_desc(uniform(s_q + q * k_bytes), 16, 1024), first_v = smem_desc(uniform(s_v), TILE_CHUNK, 1024);
+            const uint32_t desc_q = (uint32_t)first_q, desc_k = (uint32_t)smem_desc(uniform(s_k), 16, 1024), high_s = (uint32_t)(first_q >> 32);
+            const uint32_t desc_v = (uint32_t)first_v, high_v = (uint32_t)(first_v >> 32), tmem_s = uniform(tmem_base + q * 128), tmem_o = tmem_s + 256, ub = uniform(bars);
+            const uint32_t u_s = ub + 80 + 8 * q, u_pv = ub + 128 + 8 * q, u_ke = ub + 32, u_ve = ub + 64, u_qe = ub + 8;
+            const uint32_t ksteps = KS ? KS : a.dim / 16;
+            uint32_t nq = 0, nk = 0, nv = 0, np = 0;
             bool ok = true;
-            // the next scores go where the weights are, behind the product that reads them (see product_ss)
-            auto scores = [&](uint32_t q) {
-                const uint32_t dq = desc_q + q * (k_bytes >> 4), dk = desc_k + (nk & 1u) * (k_bytes >> 4), d = tmem_base + q * 128;
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) {
-                    const uint32_t off = (k >> 2) * (TILE_CHUNK >> 4) + 2 * (k & 3u);
-                    if (k < ksteps) product_ss(d, dq + off, high_s, dk + off, high_s, idesc_s, k != 0);
-                }
-                umma_commit(bar_s + 8 * q);
-            };
+            auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, pt_wait(bar, parity, s_abort, a.status)); };
             for (uint32_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-                const Item it = item_of(i);
-                if (it.tiles == 0) continue;
-                ok = pt_wait(bar_q_full, nq & 1u, s_abort, a.status);
+                const PackedItem it = item_of(i);
+                const uint32_t from = uniform(it.from[q]), to = uniform(it.to[q]), left = uniform(it.left[q]), tiles = uniform(it.tiles);
+                if (tiles == 0) continue;
+                ok = wait(bar_q_full, nq & 1u);
                 ++nq;
-                for (uint32_t t = 0; t <= it.tiles && ok; ++t) {
-                    // the products of key tile t - 1, the scores of key tile t
-                    if (t < it.tiles) ok = pt_wait(bar_k_full + 8 * (nk & 1u), (nk >> 1) & 1u, s_abort, a.status);
-                    if (t > 0) ok = ok && pt_wait(bar_v_full + 8 * (nv & 1u), (nv >> 1) & 1u, s_abort, a.status);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                    for (uint32_t q = 0; q < 2; ++q) {
-                        if (!ok) break;
-                        if (t > it.from[q] && t <= it.to[q]) {
-                            const uint32_t tmem_p = tmem_base + q * 128, d = tmem_base + 256 + q * 128, dv = desc_v + (nv & 1u) * (v_bytes >> 4);
-                            const uint32_t more = t - 1 > it.from[q];
+                for (uint32_t t = 0; t <= tiles && ok; ++t) {
+                    // the product of key tile t - 1, the scores of key tile t
+                    if (t > 0) {
+                        ok = wait(bar_v_full + 8 * (nv & 1u), (nv >> 1) & 1u);
+                        if (ok && t > from && t <= to) {
+                            const uint32_t dv = desc_v + (nv & 1u) * (v_bytes >> 4), more = t - 1 > from;
                             // keys past the last one any row of the tile sees have no weight: whole steps of them are left out
-                            const uint32_t steps = min(8u, (it.end[q] - it.anchor - (t - 1) * 128 + 15) / 16);
-                            ok = pt_wait(bar_pa + 8 * q, np[q] & 1u, s_abort, a.status);
+                            const uint32_t steps = min(8u, (left - (t - 1) * 128 + 15) / 16);
+                            ok = wait(bar_pa + 8 * q, np & 1u);
                             if (!ok) break;
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-                            for (uint32_t k = 0; k < 4; ++k)
-                                if (k < steps) product_ts(d, tmem_p + k * 8, dv + 128 * k, high_v, idesc_o, k | more);
-                            ok = pt_wait(bar_pb + 8 * q, np[q] & 1u, s_abort, a.status);
+                            for (uint32_t k = 0; k < 4; ++k) elected_ts(elected & (uint32_t)(k < steps), tmem_o, tmem_s + k * 8, dv + 128 * k, high_v, idesc_o, k | more);
+                            ok = wait(bar_pb + 8 * q, np & 1u);
                             if (!ok) break;
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-                            for (uint32_t k = 4; k < 8; ++k)
-                                if (k < steps) product_ts(d, tmem_p + k * 8, dv + 128 * k, high_v, idesc_o, 1);
-                            ++np[q];
-                            if (t == it.to[q]) umma_commit(bar_pv + 8 * q);
+                            for (uint32_t k = 4; k < 8; ++k) elected_ts(elected & (uint32_t)(k < steps), tmem_o, tmem_s + k * 8, dv + 128 * k, high_v, idesc_o, 1);
+                            ++np;
+                            if (t == to) elected_commit(elected, u_pv);
                         }
-                        if (t >= it.from[q] && t < it.to[q]) scores(q);
+                    }
+                    if (ok && t < tiles) {
+                        ok = wait(bar_k_full + 8 * (nk & 1u), (nk >> 1) & 1u);
+                        if (ok && t >= from && t < to) {
+                            // the next scores go where the weights are, behind the product that reads them (see product_ss)
+                            const uint32_t dk = desc_k + (nk & 1u) * (k_bytes >> 4);
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                            for (uint32_t k = 0; k < (KS ? KS : 8); ++k) {
+                                const uint32_t off = (k >> 2) * (TILE_CHUNK >> 4) + 2 * (k & 3u);
+                                elected_ss(KS ? elected : elected & (uint32_t)(k < ksteps), tmem_s, desc_q + off, high_s, dk + off, high_s, idesc_s, k != 0);
+                            }
+                            elected_commit(elected, u_s);
+                        }
                     }
                     if (!ok) break;
                     if (t > 0) {
-                        umma_commit(bar_v_empty + 8 * (nv & 1u));
+                        elected_commit(elected, u_ve + 8 * (nv & 1u));
                         ++nv;
                     }
-                    if (t < it.tiles) {
-                        umma_commit(bar_k_empty + 8 * (nk & 1u));
+                    if (t < tiles) {
+                        elected_commit(elected, u_ke + 8 * (nk & 1u));
                         ++nk;
-                        if (t + 1 == it.tiles) umma_commit(bar_q_empty);
+                        if (t + 1 == tiles) elected_commit(elected, u_qe);
                     }
                 }
             }
         }
-    } else {
+    } else if (warp >= 4) {
         // ---------------- softmax (TMEM lane quarter = warp % 4), then the output ----------------
-        const uint32_t q = (warp - 2) >> 2, quarter = warp & 3u, lanes = (quarter * 32u) << 16;
+        const uint32_t q = (warp - 4) >> 2, quarter = warp & 3u, lanes = (quarter * 32u) << 16;
         const uint32_t tmem_s = tmem_base + q * 128 + lanes, tmem_o = tmem_base + 256 + q * 128 + lanes;
         const uint64_t c2 = pair(p.to_log2, p.to_log2);
         uint32_t ns = 0, ndone = 0;
         bool ok = true;
         for (uint32_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-            const Item it = item_of(i);
+            const PackedItem it = item_of(i);
             const uint32_t from = q ? it.from[1] : it.from[0], to = q ? it.to[1] : it.to[0];
             if (from == to) continue;
             const uint32_t row = it.row0 + q * 128 + quarter * 32 + lane;
@@ -456,14 +489,14 @@ int32_t make_packed_map(CUtensorMap* map, const void* ptr, uint32_t width, uint3
     return HOLO_OK;
 }
 
-template <bool F16>
+template <bool F16, int KS>
 int32_t launch_packed_tile(holo_b200_ctx* ctx, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PackedTileParams& p, uint32_t grid, uint32_t smem) {
     static thread_local int configured_device = -1;
     if (configured_device != ctx->device) {
-        HOLO_CUDA(cudaFuncSetAttribute(packed_tile_kernel<F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, ctx->smem_optin));
+        HOLO_CUDA(cudaFuncSetAttribute(packed_tile_kernel<F16, KS>, cudaFuncAttributeMaxDynamicSharedMemorySize, ctx->smem_optin));
         configured_device = ctx->device;
     }
-    HOLO_CUDA(holo_launch_kernel(ctx, packed_tile_kernel<F16>, dim3(grid), dim3(PT_WARPS * 32), smem, 1, mq, mk, mv, p));
+    HOLO_CUDA(holo_launch_kernel(ctx, packed_tile_kernel<F16, KS>, dim3(grid), dim3(PT_WARPS * 32), smem, 1, mq, mk, mv, p));
     ctx->launches++;
     return HOLO_OK;
 }
@@ -491,8 +524,12 @@ int32_t holo_try_packed_tile(holo_b200_ctx* ctx, const HoloPackedArgs& a, bool* 
     HOLO_TRY(make_packed_map(&mk, a.k, a.dim, a.kv_heads, a.rows, a.k_ld));
     HOLO_TRY(make_packed_map(&mv, a.v, a.vdim, a.kv_heads, a.rows, a.v_ld));
     const uint32_t kept = a.sequences < PT_STARTS ? 4 * (a.sequences + 1) : 0;
-    const uint32_t smem = 1024 + (p.nq + 2) * p.k_chunks * TILE_CHUNK + 2 * p.v_chunks * TILE_CHUNK + 256 + ((kept + 15u) & ~15u);
+    const uint32_t smem = 1024 + (p.nq + 2) * p.k_chunks * TILE_CHUNK + 2 * p.v_chunks * TILE_CHUNK + 256 + PT_ITEMS * (uint32_t)sizeof(PackedItem) + ((kept + 15u) & ~15u);
     const uint32_t grid = p.items < (uint32_t)ctx->sm_count ? p.items : (uint32_t)ctx->sm_count;
     *taken = true;
-    return a.dtype == HOLO_DTYPE_F16 ? launch_packed_tile<true>(ctx, mq, mk, mv, p, grid, smem) : launch_packed_tile<false>(ctx, mq, mk, mv, p, grid, smem);
+    if (a.dtype == HOLO_DTYPE_F16)
+        return a.dim == 128 ? launch_packed_tile<true, 8>(ctx, mq, mk, mv, p, grid, smem)
+               : a.dim == 64 ? launch_packed_tile<true, 4>(ctx, mq, mk, mv, p, grid, smem) : launch_packed_tile<true, 0>(ctx, mq, mk, mv, p, grid, smem);
+    return a.dim == 128 ? launch_packed_tile<false, 8>(ctx, mq, mk, mv, p, grid, smem)
+           : a.dim == 64 ? launch_packed_tile<false, 4>(ctx, mq, mk, mv, p, grid, smem) : launch_packed_tile<false, 0>(ctx, mq, mk, mv, p, grid, smem);
 }
