@@ -23,6 +23,7 @@ namespace {
 
 constexpr int PT_WARPS = 12;
 constexpr uint32_t PT_ITEMS = 128;       // items of a CTA that are worked out beforehand
+constexpr uint32_t PT_SORTED = 256;      // pairs that are put in the order of their work
 constexpr float PT_GROWTH = 8.0f;
 constexpr uint32_t PT_STARTS = 4096;      // starts kept in shared memory; more are read where they are
 
@@ -61,8 +62,10 @@ __device__ __forceinline__ void elected_commit(uint32_t elected, uint32_t bar) {
 }
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 
-// An item: the query tiles of a pair (the last ones first: in a long causal sequence they have the most keys) and a head. Tile q walks the
-// key tiles [from[q], to[q]) of 128 keys each, counted from `anchor`; left[q]: keys from there to its last one.
+// An item: the query tiles of a pair and a head. Tile q walks the key tiles [from[q], to[q]) of 128 keys each, counted from `anchor`;
+// left[q]: keys from there to its last one. Pairs come in the order of their work, the most first (many pairs: the last rows
+// first, which have the most keys in a causal sequence), and CTAs take items back and forth: within 5 % of always giving the next
+// item to the CTA with the least (8192 rows of seven sequences, 1024 items: 104.5 key tiles at most for 99.5 on average; as the rows come 116.5).
 struct PackedItem {
     uint32_t row0, head, anchor, tiles, from[2], to[2], left[2];
 };
@@ -175,7 +178,9 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sm + (bars - base) + 160);
     volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(sm + (bars - base) + 164);
     PackedItem* s_items = reinterpret_cast<PackedItem*>(sm + (bars - base) + 256);
-    int32_t* s_starts = reinterpret_cast<int32_t*>(sm + (bars - base) + 256 + PT_ITEMS * sizeof(PackedItem));
+    uint32_t* s_work = reinterpret_cast<uint32_t*>(sm + (bars - base) + 256 + PT_ITEMS * sizeof(PackedItem));
+    uint16_t* s_order = reinterpret_cast<uint16_t*>(s_work + PT_SORTED);
+    int32_t* s_starts = reinterpret_cast<int32_t*>(s_order + PT_SORTED);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(bar_q_full, 1);
@@ -210,10 +215,30 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const uint32_t tmem_base = *s_tmem;
     const int32_t* starts = kept ? s_starts : a.starts;
 
+    if (p.pairs <= PT_SORTED) {
+        uint32_t mine = 0;
+        if (threadIdx.x < p.pairs) {
+            for (uint32_t q = 0; q < p.nq; ++q) {
+                const KeyRange r = keys_of_tile(a, starts, (threadIdx.x * p.nq + q) * 128);
+                mine = max(mine, r.end - r.begin);
+            }
+            s_work[threadIdx.x] = mine;
+        }
+        __syncthreads();
+        if (threadIdx.x < p.pairs) {
+            uint32_t rank = 0;
+            for (uint32_t j = 0; j < p.pairs; ++j) rank += s_work[j] > mine || (s_work[j] == mine && j < threadIdx.x);
+            s_order[rank] = (uint16_t)threadIdx.x;
+        }
+        __syncthreads();
+    }
+    const uint32_t rounds = (p.items + gridDim.x - 1) / gridDim.x;
+    // the item of this CTA's round, or one past the last
+    auto number_of = [&](uint32_t round) { return round * gridDim.x + (round & 1u ? gridDim.x - 1 - blockIdx.x : blockIdx.x); };
     auto make_item = [&](uint32_t i) {
         PackedItem it;
         it.head = i % a.heads;
-        it.row0 = (p.pairs - 1 - i / a.heads) * p.nq * 128;
+        it.row0 = (p.pairs <= PT_SORTED ? s_order[i / a.heads] : p.pairs - 1 - i / a.heads) * p.nq * 128;
         KeyRange r[2];
         r[0] = keys_of_tile(a, starts, it.row0);
         r[1] = p.nq == 2 ? keys_of_tile(a, starts, it.row0 + 128) : KeyRange{0, 0};
@@ -230,11 +255,17 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         return it;
     };
     // a thread an item
-    if (threadIdx.x < PT_ITEMS && blockIdx.x + threadIdx.x * gridDim.x < p.items) s_items[threadIdx.x] = make_item(blockIdx.x + threadIdx.x * gridDim.x);
+    if (threadIdx.x < PT_ITEMS && threadIdx.x < rounds) {
+        const uint32_t i = number_of(threadIdx.x);
+        if (i < p.items) s_items[threadIdx.x] = make_item(i);
+        else s_items[threadIdx.x].tiles = s_items[threadIdx.x].from[0] = s_items[threadIdx.x].to[0] = s_items[threadIdx.x].from[1] = s_items[threadIdx.x].to[1] = 0;
+    }
     __syncthreads();
-    auto item_of = [&](uint32_t i) {
-        const uint32_t n = (i - blockIdx.x) / gridDim.x;
-        return n < PT_ITEMS ? s_items[n] : make_item(i);
+    auto item_of = [&](uint32_t round) {
+        if (round < PT_ITEMS) return s_items[round];
+        const uint32_t i = number_of(round);
+        if (i < p.items) return make_item(i);
+        return PackedItem{};
     };
 
     if (warp == 0) {
@@ -242,7 +273,7 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (lane == 0) {
             uint32_t nq = 0, nk = 0, nv = 0;       // copies of each kind so far
             bool ok = true;
-            for (uint32_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+            for (uint32_t i = 0; i < rounds && ok; ++i) {
                 const PackedItem it = item_of(i);
                 if (it.tiles == 0) continue;
                 const int g = (int)(it.head / (a.heads / a.kv_heads));
@@ -293,7 +324,7 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             uint32_t nq = 0, nk = 0, nv = 0, np = 0;
             bool ok = true;
             auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, pt_wait(bar, parity, s_abort, a.status)); };
-            for (uint32_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+            for (uint32_t i = 0; i < rounds && ok; ++i) {
                 const PackedItem it = item_of(i);
                 const uint32_t from = uniform(it.from[q]), to = uniform(it.to[q]), left = uniform(it.left[q]), tiles = uniform(it.tiles);
                 if (tiles == 0) continue;
@@ -355,7 +386,7 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         const uint64_t c2 = pair(p.to_log2, p.to_log2);
         uint32_t ns = 0, ndone = 0;
         bool ok = true;
-        for (uint32_t i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+        for (uint32_t i = 0; i < rounds && ok; ++i) {
             const PackedItem it = item_of(i);
             const uint32_t from = q ? it.from[1] : it.from[0], to = q ? it.to[1] : it.to[0];
             if (from == to) continue;
@@ -379,19 +410,23 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 for (int c = 1; c < 4; ++c) tmem_ld32_pass(v[c]);
                 const uint32_t key0 = it.anchor + t * 128;
                 if (key0 < all_from || key0 + 128 > all_to) {
-                    // of the tile's keys this row sees [lo, hi)
+                    // of the tile's keys this row sees [lo, hi): 32 bits a request
                     const uint32_t lo = begin > key0 ? begin - key0 : 0u, hi = end > key0 ? end - key0 : 0u;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t from_lo = lo <= 32u * c ? 0xffffffffu : lo >= 32u * c + 32 ? 0u : 0xffffffffu << (lo - 32u * c);
+                        const uint32_t to_hi = hi <= 32u * c ? 0u : hi >= 32u * c + 32 ? 0xffffffffu : (1u << (hi - 32u * c)) - 1u;
+                        const uint32_t sees = from_lo & to_hi;
 #pragma unroll
                         for (int x = 0; x < 32; ++x)
-                            if (c * 32 + x < lo || c * 32 + x >= hi) v[c][x] = 0xff800000u;
+                            if (!(sees >> x & 1u)) v[c][x] = 0xff800000u;
+                    }
                 }
                 float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int x = 0; x < 32; ++x)
+                for (int x = 0; x < 32; x += 2)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) most[c] = fmaxf(most[c], __uint_as_float(v[c][x]));
+                    for (int c = 0; c < 4; ++c) most[c] = fmaxf(fmaxf(most[c], __uint_as_float(v[c][x])), __uint_as_float(v[c][x + 1]));
                 const float here = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.to_log2;
                 const bool grows = here > top + PT_GROWTH;
                 if (__any_sync(0xffffffffu, grows)) {
@@ -524,7 +559,7 @@ int32_t holo_try_packed_tile(holo_b200_ctx* ctx, const HoloPackedArgs& a, bool* 
     HOLO_TRY(make_packed_map(&mk, a.k, a.dim, a.kv_heads, a.rows, a.k_ld));
     HOLO_TRY(make_packed_map(&mv, a.v, a.vdim, a.kv_heads, a.rows, a.v_ld));
     const uint32_t kept = a.sequences < PT_STARTS ? 4 * (a.sequences + 1) : 0;
-    const uint32_t smem = 1024 + (p.nq + 2) * p.k_chunks * TILE_CHUNK + 2 * p.v_chunks * TILE_CHUNK + 256 + PT_ITEMS * (uint32_t)sizeof(PackedItem) + ((kept + 15u) & ~15u);
+    const uint32_t smem = 1024 + (p.nq + 2) * p.k_chunks * TILE_CHUNK + 2 * p.v_chunks * TILE_CHUNK + 256 + PT_ITEMS * (uint32_t)sizeof(PackedItem) + 6 * PT_SORTED + ((kept + 15u) & ~15u);
     const uint32_t grid = p.items < (uint32_t)ctx->sm_count ? p.items : (uint32_t)ctx->sm_count;
     *taken = true;
     if (a.dtype == HOLO_DTYPE_F16)
