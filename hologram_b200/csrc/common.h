@@ -405,6 +405,8 @@ struct HoloPackedArgs {
 int32_t holo_launch_packed_attention(holo_b200_ctx* ctx, const HoloPackedArgs& a);
 // packed_tile.cu: 16-bit sequences, dims in steps of 16 up to 128; *taken false: the shape is not one it serves
 int32_t holo_try_packed_tile(holo_b200_ctx* ctx, const HoloPackedArgs& a, bool* taken);
+// packed_f32.cu: f32 sequences, dims in steps of 4 up to 128
+int32_t holo_try_packed_f32(holo_b200_ctx* ctx, const HoloPackedArgs& a, bool* taken);
 // block_cache.cu: the cache's operands, shared by its two calls
 struct HoloBlockCache {
     const int32_t *starts, *lengths, *table;     // starts null: row s is sequence s's only one

@@ -39,6 +39,8 @@ int32_t holo_launch_packed_attention(holo_b200_ctx* ctx, const HoloPackedArgs& a
     bool taken;
     HOLO_TRY(holo_try_packed_tile(ctx, a, &taken));
     if (taken) return HOLO_OK;
+    HOLO_TRY(holo_try_packed_f32(ctx, a, &taken));
+    if (taken) return HOLO_OK;
     PackedSource src = {a};
     return launch_general_rows(ctx, src, (uint64_t)a.rows * a.heads, a.vdim);
 }
