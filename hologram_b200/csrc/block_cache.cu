@@ -12,12 +12,11 @@ namespace {
 // The integer nearest to x / s, ties to even, for s > 0, clamped to +-127. An estimate that is at most one off, and the exact remainder
 // of x by it: x - n s is a multiple of the smaller of the two's last places and smaller than 2 s, so fma holds it, or rounds it on the same side of +-s / 2.
 __device__ __forceinline__ int nearest_code(float x, float s, float inv) {
-    float n = rintf(x * inv);
-    const float r = fmaf(-n, s, x), twice = 2.0f * r;
-    const bool odd = ((int)n & 1) != 0;
-    if (twice > s || (twice == s && odd)) n += 1.0f;
-    if (twice < -s || (twice == -s && odd)) n -= 1.0f;
-    return max(-127, min(127, __float2int_rn(n)));
+    const float n = rintf(x * inv), r = fmaf(-n, s, x), twice = 2.0f * r;
+    int i = __float2int_rn(n);
+    // further than half a step, or just there from an odd number: the other neighbour
+    if (fabsf(twice) > s || (fabsf(twice) == s && (i & 1))) i += r > 0.0f ? 1 : -1;
+    return max(-127, min(127, i));
 }
 // The same in 64 bits for x and s of 31 bits at most, whose remainder is exact there; about = x / s, rounded somehow.
 __device__ __forceinline__ int nearest_code(double x, double s, double about) {
@@ -36,13 +35,79 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
 }
 
 constexpr int WRITE_THREADS = 128;
+constexpr int WRITE_KEPT = 4;       // units of new values a thread keeps from the search for the largest to the coding
 
-__global__ void __launch_bounds__(WRITE_THREADS)
+// VEC values of a row at a time (8 where rows and pitches allow 16-byte loads of 16-bit types, 4 of f32, else 1), kept as they came
+template <int VEC>
+struct Unit {
+    uint4 raw;
+};
+template <>
+struct Unit<1> {
+    float raw;
+};
+template <int DT, int VEC>
+__device__ __forceinline__ Unit<VEC> load_unit(const void* p, uint64_t i) {
+    Unit<VEC> u;
+    if constexpr (VEC == 1) u.raw = seq_load(p, i, DT);
+    else u.raw = *reinterpret_cast<const uint4*>((const uint8_t*)p + i * (16 / VEC));
+    return u;
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void values_of(const Unit<VEC>& u, float (&x)[VEC]) {
+    if constexpr (VEC == 1) {
+        x[0] = u.raw;
+    } else {
+        const uint32_t w[4] = {u.raw.x, u.raw.y, u.raw.z, u.raw.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (DT == HOLO_DTYPE_F32) {
+                x[e] = __uint_as_float(w[e]);
+            } else if constexpr (DT == HOLO_DTYPE_BF16) {
+                x[2 * e] = __uint_as_float(w[e] << 16);
+                x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+            } else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                x[2 * e] = f.x;
+                x[2 * e + 1] = f.y;
+            }
+        }
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void store_codes(int8_t* to, const int (&code)[VEC]) {
+    if (VEC == 1) {
+        *to = (int8_t)code[0];
+    } else {
+        uint32_t w[(VEC + 3) / 4];
+#pragma unroll
+        for (int e = 0; e < (VEC + 3) / 4; ++e)
+            w[e] = __byte_perm(__byte_perm((uint32_t)code[(4 * e) % VEC], (uint32_t)code[(4 * e + 1) % VEC], 0x0040),
+                               __byte_perm((uint32_t)code[(4 * e + 2) % VEC], (uint32_t)code[(4 * e + 3) % VEC], 0x0040), 0x5410);
+        if (VEC == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[(VEC + 3) / 4 - 1]);
+        else *reinterpret_cast<uint32_t*>(to) = w[0];
+    }
+}
+
+// What a block held in a smaller scale, said in the new one.
+__device__ __noinline__ void recode_rows(int8_t* codes, uint32_t n, float before, float now) {
+    const double ratio = (double)before / (double)now;
+    for (uint32_t i = threadIdx.x; i < n; i += WRITE_THREADS) {
+        const double old = (double)codes[i];
+        codes[i] = (int8_t)nearest_code(old * (double)before, (double)now, old * ratio);
+    }
+}
+__device__ __noinline__ int any_code(float x, float s, float inv) { return code_of(x, s, inv); }
+
+// 128-thread CTAs, eight to an SM: what a CTA waits for is a chain of loads (starts, length, block number, rows), hidden by the others
+template <int DT, int VEC>
+__global__ void __launch_bounds__(WRITE_THREADS, 8)
 block_write_kernel(const __grid_constant__ HoloBlockWriteArgs a) {
-    __shared__ float s_most[WRITE_THREADS / 32];
+    __shared__ uint32_t s_most[WRITE_THREADS / 32];
     const HoloBlockCache& c = a.c;
-    const uint32_t item = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, br = c.block_rows;
-    const bool values = blockIdx.z != 0;
+    // neighbouring CTAs take the heads of the same rows, whose values lie side by side
+    const uint32_t head = blockIdx.x % c.kv_heads, item = blockIdx.x / c.kv_heads >> 1, tid = threadIdx.x, br = c.block_rows;
+    const bool values = (blockIdx.x / c.kv_heads & 1u) != 0;
     holo_pdl_trigger();
     holo_pdl_wait();
     const int64_t most = (int64_t)c.table_ld * br;
@@ -51,19 +116,23 @@ block_write_kernel(const __grid_constant__ HoloBlockWriteArgs a) {
     uint32_t s, nth;
     int64_t begin, count;
     if (c.starts) {
-        int lo = -1, hi = (int)c.sequences - 1;
-        while (lo < hi) {
-            const int mid = lo + (hi - lo + 1) / 2;
-            if ((int64_t)(max(c.starts[mid], 0) / (int)br) + 2ll * mid <= (int64_t)item) lo = mid;
-            else hi = mid - 1;
+        // the last sequence whose first item is at most `item`: 32 places a round trip
+        uint32_t lo = 0, left = c.sequences;
+        while (left > 0) {
+            const uint32_t step = (left + 31) / 32, at = lo + min(tid & 31u, (left - 1) / step) * step;
+            const bool below = (int64_t)((uint32_t)max(c.starts[at], 0) / br) + 2ll * at <= (int64_t)item;
+            const uint32_t ahead = __ballot_sync(0xffffffffu, below);
+            if (ahead == 0) return;         // starts that do not begin at 0
+            lo = __shfl_sync(0xffffffffu, at, 31 - __clz(ahead));
+            if (step == 1) break;
+            left = min(step, c.sequences - lo);
         }
-        if (lo < 0) return;
-        s = (uint32_t)lo;
+        s = lo;
         begin = c.starts[s];
         const int64_t end = c.starts[s + 1];
         if (begin < 0 || end > c.rows) return;
         count = end - begin;
-        nth = item - (uint32_t)(begin / br) - 2 * s;
+        nth = item - (uint32_t)begin / br - 2 * s;
     } else {
         s = item;
         begin = s;
@@ -72,43 +141,87 @@ block_write_kernel(const __grid_constant__ HoloBlockWriteArgs a) {
     }
     const int64_t length = c.lengths[s], first = length - count;
     if (count <= 0 || first < 0 || length > most) return;
-    const uint32_t j = (uint32_t)(first / br) + nth;
-    const int64_t block_at = (int64_t)j * br;
-    if (block_at >= length) return;
+    const uint32_t j = (uint32_t)first / br + nth, block_at = j * br;      // positions are below 2^31
+    if ((int64_t)block_at >= length) return;
     const int id = c.table[(uint64_t)s * c.table_ld + j];
     if (id < 0 || (uint32_t)id >= c.blocks) {
         if (tid == 0) atomicOr(c.status, HOLO_STATUS_TABLE);
         return;
     }
-    const uint32_t lo = first > block_at ? (uint32_t)(first - block_at) : 0u, hi = (uint32_t)min((int64_t)br, length - block_at);     // new rows of the block
+    const uint32_t lo = first > block_at ? (uint32_t)first - block_at : 0u, hi = (uint32_t)min((int64_t)br, length - block_at);     // new rows of the block
     const uint32_t d = values ? c.vdim : c.dim, ld = values ? a.v_ld : a.k_ld;
-    const void* x = values ? a.v : a.k;
     const uint64_t plane = (uint64_t)id * c.kv_heads + head;
     int8_t* codes = (values ? c.v_codes : c.k_codes) + plane * br * d;
     float* scale = (values ? c.v_scales : c.k_scales) + plane;
-    const uint64_t row0 = (uint64_t)(begin + (block_at + lo - first));      // the call's row behind the block's row `lo`
-    const uint32_t n = (hi - lo) * d;
-    float largest = 0.0f;
-    for (uint32_t i = tid; i < n; i += WRITE_THREADS) {
-        const float m = fabsf(seq_load(x, (row0 + i / d) * ld + (uint64_t)head * d + i % d, a.dtype));
-        if (m < INFINITY) largest = fmaxf(largest, m);
-    }
-    for (int o = 16; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-    if ((tid & 31) == 0) s_most[tid >> 5] = largest;
+    const void* x = values ? a.v : a.k;
+    const uint64_t x0 = (uint64_t)(begin + (block_at + lo - first)) * ld + (uint64_t)head * d;      // the block's row `lo` in the call's rows
+    const uint32_t across = d / VEC, n = (hi - lo) * across;
     const float before = lo ? *scale : 0.0f;
-    __syncthreads();        // nobody stores the new scale before everybody has read the old one
-    for (int w = 0; w < WRITE_THREADS / 32; ++w) largest = fmaxf(largest, s_most[w]);
-    const float now = fmaxf(before, __fdiv_rn(largest, 127.0f));
-    if (now > before && lo) {
-        const double ratio = (double)before / (double)now;
-        for (uint32_t i = tid; i < lo * d; i += WRITE_THREADS) {
-            const double old = (double)codes[i];
-            codes[i] = (int8_t)nearest_code(old * (double)before, (double)now, old * ratio);
+    Unit<VEC> kept[WRITE_KEPT];
+    auto unit = [&](uint32_t i) { return load_unit<DT, VEC>(x, x0 + (uint64_t)(i / across) * ld + (i % across) * VEC); };
+#pragma unroll
+    for (int u = 0; u < WRITE_KEPT; ++u)
+        if (tid + u * WRITE_THREADS < n) kept[u] = unit(tid + u * WRITE_THREADS);
+    // magnitudes order as their bits do, infinities and NaN above all
+    uint32_t largest = 0;
+    auto look = [&](const Unit<VEC>& u, uint32_t below) {
+        float v[VEC];
+        values_of<DT, VEC>(u, v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
+            if (m < below) largest = max(largest, m);
         }
+    };
+    auto look_all = [&](uint32_t below) {
+#pragma unroll
+        for (int u = 0; u < WRITE_KEPT; ++u)
+            if (tid + u * WRITE_THREADS < n) look(kept[u], below);
+#pragma unroll 1
+        for (uint32_t i = tid + WRITE_KEPT * WRITE_THREADS; i < n; i += WRITE_THREADS) look(unit(i), below);
+        largest = __reduce_max_sync(0xffffffffu, largest);
+        if ((tid & 31) == 0) s_most[tid >> 5] = largest;
+        __syncthreads();        // nobody stores the new scale before everybody has read the old one
+#pragma unroll
+        for (int w = 0; w < WRITE_THREADS / 32; ++w) largest = max(largest, s_most[w]);
+    };
+    look_all(0xffffffffu);
+    const bool finite = largest < 0x7f800000u;
+    if (!finite) {
+        __syncthreads();
+        largest = 0;
+        look_all(0x7f800000u);
     }
-    const float inv = now < 1.2e-38f ? 0.0f : __fdiv_rn(1.0f, now);
-    for (uint32_t i = tid; i < n; i += WRITE_THREADS)
-        codes[lo * d + i] = (int8_t)code_of(seq_load(x, (row0 + i / d) * ld + (uint64_t)head * d + i % d, a.dtype), now, inv);
+    const float now = fmaxf(before, __fdiv_rn(__uint_as_float(largest), 127.0f));
+    if (lo && now > before) recode_rows(codes, lo * d, before, now);
+    const float inv = now < 1.2e-37f ? 0.0f : __fdiv_rn(1.0f, now), half = 0.5f * now;
+    const bool plain = finite && inv != 0.0f;
+    auto encode = [&](uint32_t i, const Unit<VEC>& u) {
+        float v[VEC];
+        values_of<DT, VEC>(u, v);
+        int code[VEC];
+        bool special = !plain;
+        if (plain) {
+            // |x / now| is 127 at most, but for roundings: a sum with 1.5 * 2^23 has the integer next to it in its low bits. The remainder
+            // is exact (see nearest_code); just half a step away it is left to that.
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float m = fmaf(v[e], inv, 12582912.0f), r = fmaf(12582912.0f - m, now, v[e]);
+                code[e] = __float_as_int(m) + (r > half ? 1 : 0) - (r < -half ? 1 : 0);
+                special = special || fabsf(r) == half;
+            }
+        }
+        if (special) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) code[e] = any_code(v[e], now, now < 1.2e-37f ? 0.0f : inv);
+        }
+        store_codes<VEC>(codes + lo * d + i * VEC, code);
+    };
+#pragma unroll
+    for (int u = 0; u < WRITE_KEPT; ++u)
+        if (tid + u * WRITE_THREADS < n) encode(tid + u * WRITE_THREADS, kept[u]);
+#pragma unroll 1
+    for (uint32_t i = tid + WRITE_KEPT * WRITE_THREADS; i < n; i += WRITE_THREADS) encode(i, unit(i));
     if (tid == 0) *scale = now;
 }
 
@@ -158,8 +271,16 @@ struct CacheSource {
 
 int32_t holo_launch_block_cache_write(holo_b200_ctx* ctx, const HoloBlockWriteArgs& a) {
     const uint64_t items = a.c.starts ? (uint64_t)a.c.rows / a.c.block_rows + 2ull * a.c.sequences : a.c.sequences;
-    if (items > 0x7fffffffull || a.c.kv_heads > 65535) return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: block_cache_write of %u rows, %u heads", a.c.rows, a.c.kv_heads);
-    HOLO_CUDA(holo_launch_kernel(ctx, block_write_kernel, dim3((uint32_t)items, a.c.kv_heads, 2), dim3(WRITE_THREADS), 0, 1, a));
+    if (items * a.c.kv_heads > 0x3fffffffull) return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: block_cache_write of %u rows, %u heads", a.c.rows, a.c.kv_heads);
+    const uint32_t es = (uint32_t)holo_dtype_size(a.dtype), vec = 16 / es;
+    const bool wide = ((((uintptr_t)a.k | (uintptr_t)a.v) & 15u) | (a.c.dim | a.c.vdim | a.k_ld | a.v_ld) % vec) == 0 && (((uintptr_t)a.c.k_codes | (uintptr_t)a.c.v_codes) & 7u) == 0;
+    const dim3 grid((uint32_t)(items * a.c.kv_heads * 2)), block(WRITE_THREADS);
+    auto launch = [&](auto kernel) { return holo_launch_kernel(ctx, kernel, grid, block, 0, 1, a); };
+    cudaError_t e;
+    if (a.dtype == HOLO_DTYPE_F32) e = wide ? launch(block_write_kernel<HOLO_DTYPE_F32, 4>) : launch(block_write_kernel<HOLO_DTYPE_F32, 1>);
+    else if (a.dtype == HOLO_DTYPE_BF16) e = wide ? launch(block_write_kernel<HOLO_DTYPE_BF16, 8>) : launch(block_write_kernel<HOLO_DTYPE_BF16, 1>);
+    else e = wide ? launch(block_write_kernel<HOLO_DTYPE_F16, 8>) : launch(block_write_kernel<HOLO_DTYPE_F16, 1>);
+    HOLO_CUDA(e);
     ctx->launches++;
     return HOLO_OK;
 }
