@@ -101,6 +101,7 @@ extern "C" void holo_b200_ctx_destroy(holo_b200_ctx* ctx) {
     if (ctx->host_stage) cudaFreeHost(ctx->host_stage);
     if (ctx->causal_partials) cudaFree(ctx->causal_partials);
     if (ctx->block_partials) cudaFree(ctx->block_partials);
+    if (ctx->block_row_partials) cudaFree(ctx->block_row_partials);
     if (ctx->latent_partials) cudaFree(ctx->latent_partials);
     if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
     delete ctx;

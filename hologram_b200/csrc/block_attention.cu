@@ -17,8 +17,7 @@
 // that neither short sequences nor few heads leave SMs without work. Where a share begins or ends inside a plane its partial result goes
 // to a buffer of the context, and the last of the plane's CTAs to arrive adds them up in the order of the list: nobody waits,
 // and no order of arrival shows in the result.
-#include "attention_tile.cuh"
-#include "sequences.cuh"
+#include "block_list.cuh"
 
 namespace {
 
@@ -34,90 +33,11 @@ struct BlockAttnParams {
     bool aligned_out;
 };
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ float2 half_values(uint32_t v) {
-    float2 r;
-    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.f32.f16 %0, l;\ncvt.f32.f16 %1, h;\n}" : "=f"(r.x), "=f"(r.y) : "r"(v));
-    return r;
-}
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Bytes 0 and 2 (1 and 3) of four codes plus 128 as a pair of f16 codes
-template <uint32_t PICK>
-__device__ __forceinline__ uint32_t codes_to_half(uint32_t biased) {
-    const uint32_t raised = __byte_perm(biased, 0x64646464u, PICK);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&raised), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-constexpr uint32_t PICK02 = 0x4240, PICK13 = 0x4341;
-
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool take) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4u : 0u) : "memory");
-}
-
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
-// The list of planes: sequence by sequence, kv head by kv head, R rows by R rows; `at` counts the slabs of all planes before.
-struct Plane {
-    uint32_t seq, head, tile, tiles, first_row, n, slabs, at;
-    int32_t length;
-};
-template <int R>
-__device__ __forceinline__ uint32_t rows_before(const Plane& p, uint32_t tile, uint32_t group) {       // positions up to the tile's last one
-    return min(p.n, (tile * R + R - 1) / group + 1);
-}
-template <int R>
-__device__ __forceinline__ uint32_t slabs_of(const Plane& p, uint32_t tile, uint32_t group) {
-    const int32_t sees = p.length - (int32_t)(p.n - rows_before<R>(p, tile, group));
-    return sees <= 0 ? 0u : ((uint32_t)sees + BA_SLAB - 1) / BA_SLAB;
-}
-template <int R>
-__device__ __forceinline__ void read_sequence(const HoloBlockCache& c, uint32_t group, uint32_t s, Plane* p) {
-    int32_t b = (int32_t)s, e = (int32_t)s + 1;
-    if (c.starts) {
-        b = c.starts[s];
-        e = c.starts[s + 1];
-        if (b < 0 || e < b || e > (int32_t)c.rows) b = e = 0;
-    }
-    p->seq = s;
-    p->first_row = (uint32_t)b;
-    p->n = (uint32_t)(e - b);
-    p->length = max(0, min(c.lengths[s], (int32_t)(c.table_ld * c.block_rows)));
-    p->tiles = (p->n * group + R - 1) / R;
-    p->head = p->tile = 0;
-}
-// On to the next plane that has slabs; slabs == 0: there is none.
-template <int R>
-__device__ __forceinline__ void next_plane(const HoloBlockCache& c, uint32_t group, Plane* p) {
-    p->at += p->slabs;
-    for (;;) {
-        if (++p->tile >= p->tiles) {
-            p->tile = 0;
-            if (++p->head >= c.kv_heads) {
-                if (++p->seq >= c.sequences) {
-                    p->slabs = 0;
-                    return;
-                }
-                read_sequence<R>(c, group, p->seq, p);
-            }
-        }
-        p->slabs = p->tiles ? slabs_of<R>(*p, p->tile, group) : 0u;
-        if (p->slabs) return;
-        if (!p->tiles) p->head = c.kv_heads - 1;
-    }
-}
-
 // RT: four query rows or eight. D: dim and vdim where both are MAXD (their steps are constants then), else 0. SECOND: eight rows' weights
 // as two terms.
 template <int RT, int MAXD, bool EXACT, bool SECOND, int STAGES, int CTAS>
@@ -137,105 +57,10 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
     holo_pdl_wait();
     if (blockIdx.x == 0) check_sequences(c.starts, c.lengths, c.sequences, c.rows, (int64_t)c.table_ld * br, c.status);
 
-    // ---- this CTA's share of the list; every warp finds it by itself, four sequences a lane at a time ----
-    uint32_t cnt[4], upto = 0, sum = 0, all = 0, planes = 0;
-    uint32_t unit = 1;              // slabs of a piece: 1, or where no CTA takes pieces of two planes, its share
-    auto count_chunk = [&](uint32_t s0) {
-        Plane seq[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t s = s0 + 4 * lane + i;
-            read_sequence<R>(c, group, min(s, c.sequences - 1), &seq[i]);
-            if (s >= c.sequences) seq[i].tiles = 0;
-        }
-        sum = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            cnt[i] = 0;
-#pragma unroll 1
-            for (uint32_t t = 0; t < seq[i].tiles; ++t) cnt[i] += (slabs_of<R>(seq[i], t, group) + unit - 1) / unit;
-            cnt[i] *= c.kv_heads;
-            sum += cnt[i];
-            planes += seq[i].tiles;
-        }
-        upto = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= (uint32_t)o) upto += u;
-        }
-        all = __shfl_sync(0xffffffffu, upto, 31);
-    };
-    uint32_t total = 0;
-#pragma unroll 1
-    for (uint32_t s0 = 0; s0 < c.sequences; s0 += 128) {
-        count_chunk(s0);
-        total += all;
-    }
-    planes = __reduce_add_sync(0xffffffffu, planes) * c.kv_heads;
-    // A share is one slab a warp at least: fewer CTAs take part in a short list. Few planes are cut into pieces of their own, at most as
-    // many as there are CTAs, where that lengthens a share by less than the 8 slabs (2 a warp) that a second plane costs a CTA.
-    const uint32_t grid = gridDim.x;
-    const bool apart = planes < grid && (uint64_t)total * planes <= 8ull * grid * (grid - planes);
-    uint32_t ctas = min(grid, (total + BA_WARPS - 1) / BA_WARPS), each = 0, more_by_one = 0, want = 0;
-    if (apart) {
-        unit = max((total + grid - planes - 1) / (grid - planes), (uint32_t)BA_WARPS);
-        want = blockIdx.x;
-    } else {
-        if (blockIdx.x >= ctas) return;
-        each = total / ctas;
-        more_by_one = total - each * ctas;
-        want = blockIdx.x * each + min(blockIdx.x, more_by_one);
-    }
-    Plane first = {};
-    uint32_t lo, hi, part = 0;      // this CTA's slabs; apart: of its plane, of which they are the part of this number
-    {
-        uint32_t run = 0, s0 = 0;
-        bool found = false;
-#pragma unroll 1
-        for (;; s0 += 128) {
-            if (apart || c.sequences > 128) count_chunk(s0);
-            found = want < run + all;
-            if (found || s0 + 128 >= c.sequences) break;
-            run += all;
-        }
-        if (!found) return;
-        uint32_t at = run + upto - sum, mine = 0, which = 0;
-        const uint32_t from = __ffs(__ballot_sync(0xffffffffu, want < run + upto)) - 1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (mine == 0) {
-                if (want < at + cnt[i]) {
-                    mine = cnt[i];
-                    which = s0 + 4 * lane + i;
-                } else {
-                    at += cnt[i];
-                }
-            }
-        which = __shfl_sync(0xffffffffu, which, from);
-        at = __shfl_sync(0xffffffffu, at, from);
-        mine = __shfl_sync(0xffffffffu, mine, from);
-        read_sequence<R>(c, group, min(which, c.sequences - 1), &first);
-        const uint32_t a_head = max(mine / c.kv_heads, 1u);
-        first.head = min((want - at) / a_head, c.kv_heads - 1);
-        first.at = at + first.head * a_head;
-        first.slabs = slabs_of<R>(first, 0, group);
-        for (;;) {
-            const uint32_t pieces = (first.slabs + unit - 1) / unit;
-            if (want < first.at + pieces || first.tile + 1 >= first.tiles) break;
-            first.at += pieces;
-            first.slabs = slabs_of<R>(first, ++first.tile, group);
-        }
-        if (apart) {
-            part = want - first.at;
-            first.at = 0;
-            lo = part * unit;
-            hi = min(lo + unit, first.slabs);
-        } else {
-            lo = want;
-            hi = (blockIdx.x + 1) * each + min(blockIdx.x + 1, more_by_one);
-        }
-    }
+    Share mine;
+    if (!find_share<R, BA_SLAB, BA_WARPS, 8>(c, group, &mine)) return;
+    const uint32_t lo = mine.lo, hi = mine.hi;
+    const Plane first = mine.first;
 
     // ---- a plane's rows: requested early, cut into digits when the plane begins ----
     constexpr int OWN = R / BA_WARPS;
@@ -261,10 +86,6 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
     // sequence's last position come along, are masked, and are integers whatever they hold.
     const bool one_block = br % BA_SLAB == 0;
     auto block_of = [&](uint32_t pos) { return p.br_shift >= 0 ? pos >> p.br_shift : pos / br; };
-    auto ends_of = [&](const Plane& q, uint32_t* s0, uint32_t* s1) {      // the slabs of a plane that are this CTA's
-        *s0 = lo > q.at ? lo - q.at : 0u;
-        *s1 = min(q.slabs, hi - q.at);
-    };
     Plane ahead = first;            // where the next slab to request lies
     uint32_t ahead_slab, ahead_end, ahead_sees, ids_at = 0;
     int ahead_id = -1, ids = -1;    // ids: the blocks from number ids_at on, one a lane
@@ -274,7 +95,7 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
         ids = blk + lane <= block_of(ahead_sees - 1) ? c.table[(uint64_t)ahead.seq * c.table_ld + blk + lane] : -1;
     };
     auto enter_ahead = [&]() {
-        ends_of(ahead, &ahead_slab, &ahead_end);
+        mine.ends_of(ahead, &ahead_slab, &ahead_end);
         ahead_slab += warp;
         ahead_sees = (uint32_t)ahead.length - (ahead.n - rows_before<R>(ahead, ahead.tile, group));
         load_ids(block_of(ahead_slab * BA_SLAB));
@@ -285,7 +106,7 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
                 more = false;
                 return;
             }
-            next_plane<R>(c, group, &ahead);
+            next_plane<R, BA_SLAB>(c, group, &ahead);
             if (!ahead.slabs) {
                 more = false;
                 return;
@@ -409,7 +230,7 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
 #pragma unroll
             for (int x = 0; x < 4; ++x) o[i][x] = 0.0f;
         uint32_t from, to;
-        ends_of(at, &from, &to);
+        mine.ends_of(at, &from, &to);
 #pragma unroll 1
         for (uint32_t slab = from + warp; slab < to; slab += BA_WARPS) {
             request(stage == 0 ? STAGES - 1 : stage - 1);      // where the slab before this one was
@@ -531,7 +352,7 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
         Plane next = at;
         const bool begins = at.at >= lo, ends = at.at + at.slabs <= hi, whole = begins && ends;
         if (at.at + at.slabs < hi) {
-            next_plane<R>(c, group, &next);
+            next_plane<R, BA_SLAB>(c, group, &next);
             if (next.slabs) load_rows(next);
         }
         float* partial = p.partials + ((uint64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * R * (vdim + 2);
@@ -590,13 +411,8 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
             }
         }
         if (!whole) {
-            // the CTAs that share the plane, and its counter: that of the CTA it begins in
-            auto owner = [&](uint32_t slab) {
-                const uint32_t longer = more_by_one * (each + 1);
-                return slab < longer ? slab / (each + 1) : more_by_one + (slab - longer) / each;
-            };
-            const uint32_t from_cta = apart ? blockIdx.x - part : owner(at.at);
-            const uint32_t count = apart ? (at.slabs + unit - 1) / unit : owner(at.at + at.slabs - 1) - from_cta + 1;
+            // the plane's CTAs, and its counter: that of the CTA it begins in
+            const uint32_t from_cta = mine.first_cta(at), count = mine.cta_count(at);
             __syncthreads();
             if (tid == 0) {
                 uint32_t n;

@@ -53,6 +53,7 @@ struct holo_b200_ctx {
     float* causal_partials = nullptr;   // split-key partials of the causal attention, allocated once at a fixed size (graphs hold its address)
     float* latent_partials = nullptr;   // the same for the latent attention
     float* block_partials = nullptr;    // partial results of the block cache's attention, allocated once at a fixed size
+    float* block_row_partials = nullptr;   // the same for its calls of many rows
     float* split_partials = nullptr;    // split-key partials of the float-cache attention (HOLO_SPLIT_PARTIAL_BYTES, made with the context) or null
     bool session_capture = false;       // the stream is recording a session's own walk: its replays are ordered on this stream too
     uint32_t* attn_arrivals = nullptr;  // 65536 counters, zero between launches (decode attention)
@@ -433,6 +434,8 @@ struct HoloBlockAttnArgs {
 int32_t holo_launch_block_cache_attention(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a);
 // block_attention.cu: dims in steps of 16; *taken false: the shape is not one it serves
 int32_t holo_try_block_attention(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool* taken);
+// block_rows.cu: many rows of a sequence
+int32_t holo_try_block_rows(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool* taken);
 // logit_rules.cu
 struct HoloLogitRulesArgs {
     const void* logits;
