@@ -1,7 +1,9 @@
 // Attention of many rows of each sequence (portions of prompts) over the int8 block cache, for dims in steps of 16 up to 128.
 //
-// A CTA takes 128 query rows of a kv head (a row is a new position and a head of the group), 16 a warp, and walks the keys in slabs of 64.
-// The codes of a slab are copied to a ring (cp.async), turned into f16 once for all eight warps (exact: integers of 8 bits), while the slab
+// A CTA takes 128 query rows of a kv head (a row is a new position and a head of the group) and walks the keys in slabs of 64; two warps share
+// 16 rows, each with half of a slab's keys and a maximum, sums and a context of its own, joined at the plane's end: sixteen warps hide more
+// of each other's latency than eight with whole slabs (000 us against 472 for the portions below).
+// The codes of a slab are copied to a ring (cp.async), turned into f16 once for all warps (exact: integers of 8 bits), while the slab
 // before is worked on, and are the operands of mma.sync m16n8k16 with f32 sums. Query rows are scaled by a power of two to a largest value in
 // [2^14, 2^15), so that bf16 and f16 queries are exact in f16 (values 2^29 smaller than the largest aside); f32 queries go as two f16 terms,
 // which hold 22 bits. Scales of blocks are applied to the scores, and to the weights, w = 2^(s - max) * scale_v relative to a power of two that
@@ -12,7 +14,7 @@
 
 namespace {
 
-constexpr int BR_ROWS = 128, BR_SLAB = 64, BR_WARPS = 8, BR_STAGES = 3;
+constexpr int BR_ROWS = 128, BR_SLAB = 64, BR_WARPS = 16, BR_STAGES = 3;
 constexpr uint32_t BR_THREADS = BR_WARPS * 32;
 
 struct BlockRowsParams {
@@ -28,14 +30,14 @@ constexpr uint32_t PICK01 = 0x4140, PICK23 = 0x4342;
 template <int MAXD, bool TWO>
 __global__ void __launch_bounds__(BR_THREADS, 1)
 block_rows_kernel(const __grid_constant__ BlockRowsParams p) {
-    constexpr int KSTEPS = MAXD / 16, CHUNKS = MAXD / 16, UNITS = BR_SLAB * MAXD / 16 / BR_THREADS;      // 16-byte units of codes a thread
+    constexpr int KSTEPS = MAXD / 16, CHUNKS = MAXD / 16, UNITS = (BR_SLAB * MAXD / 16 + BR_THREADS - 1) / BR_THREADS, KEYS = BR_SLAB / 2;      // 16-byte units of codes a thread
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_row[BR_ROWS], s_scales[4][2][BR_SLAB];
     __shared__ uint32_t s_last;
     const HoloBlockAttnArgs& a = p.a;
     const HoloBlockCache& c = a.c;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane >> 2, in_quad = lane & 3;
-    const uint32_t group = p.group, dim = c.dim, vdim = c.vdim, br = c.block_rows, k_chunks = dim / 16, v_chunks = vdim / 16;
+    const uint32_t rows16 = warp & 7u, half = warp >> 3, group = p.group, dim = c.dim, vdim = c.vdim, br = c.block_rows, k_chunks = dim / 16, v_chunks = vdim / 16;
     const uint32_t q_at = smem_u32(smem), tiles_at = q_at + p.q_bytes, ring_at = tiles_at + 2 * p.tile_bytes;
     uint8_t *tiles_mem = smem + p.q_bytes, *ring_mem = tiles_mem + 2 * p.tile_bytes;
     holo_pdl_trigger();
@@ -129,7 +131,7 @@ block_rows_kernel(const __grid_constant__ BlockRowsParams p) {
         for (uint32_t s = 0; s < BR_STAGES; ++s) request(s0 + s);
         // ---- the rows of the plane, a warp its own ----
 #pragma unroll 4
-        for (uint32_t r = warp * 16; r < warp * 16 + 16; ++r) {
+        for (uint32_t r = warp * 8; r < warp * 8 + 8; ++r) {
             const uint32_t flat = at.tile * BR_ROWS + r, i = flat / group, head = at.head * group + flat % group;
             float x[MAXD / 32], most = 0.0f;
             bool finite = true;
@@ -157,13 +159,14 @@ block_rows_kernel(const __grid_constant__ BlockRowsParams p) {
             }
             if (lane == 0) s_row[r] = finite ? a.scale * LOG2E * power_of_two(-(up / 2)) * power_of_two(-(up - up / 2)) : NAN;
         }
-        __syncwarp();
-        const bool works = warp * 16 < rows;
-        const float row_scale[2] = {s_row[warp * 16 + quad], s_row[warp * 16 + quad + 8]};
+        asm volatile("cp.async.wait_group %0;" ::"n"(BR_STAGES - 1) : "memory");
+        __syncthreads();
+        const bool works = rows16 * 16 < rows;
+        const float row_scale[2] = {s_row[rows16 * 16 + quad], s_row[rows16 * 16 + quad + 8]};
         uint32_t limit[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const uint32_t i = (at.tile * BR_ROWS + min(warp * 16 + quad + 8 * x, rows - 1)) / group;
+            const uint32_t i = (at.tile * BR_ROWS + min(rows16 * 16 + quad + 8 * x, rows - 1)) / group;
             limit[x] = (uint32_t)max(0, at.length - (int32_t)(at.n - i - 1));
         }
         // keys that all rows of the warp see, and that any does
@@ -174,8 +177,6 @@ block_rows_kernel(const __grid_constant__ BlockRowsParams p) {
         for (int i = 0; i < CHUNKS; ++i)
 #pragma unroll
             for (int x = 0; x < 4; ++x) o[i][0][x] = o[i][1][x] = 0.0f;
-        asm volatile("cp.async.wait_group %0;" ::"n"(BR_STAGES - 1) : "memory");
-        __syncthreads();
         convert(s0);
 #pragma unroll 1
         for (uint32_t slab = s0; slab < s1; ++slab) {
@@ -183,49 +184,58 @@ block_rows_kernel(const __grid_constant__ BlockRowsParams p) {
             __syncthreads();        // the next slab's codes are here, this one's f16 are, and everybody has left the one before
             convert(slab + 1);
             request(slab + BR_STAGES);
-            if (!works || slab * BR_SLAB >= most_keys) continue;
-            const uint32_t k_at = tiles_at + ((slab - s0) & 1u) * p.tile_bytes, v_at = k_at + BR_SLAB * p.k_pitch;
-            const float *ks = s_scales[(slab - s0) & 3u][0], *vs = s_scales[(slab - s0) & 3u][1];
-            float s[8][4];
+            if (!works || slab * BR_SLAB + half * KEYS >= most_keys) continue;
+            const uint32_t k_at = tiles_at + ((slab - s0) & 1u) * p.tile_bytes + half * KEYS * p.k_pitch;
+            const uint32_t v_at = tiles_at + ((slab - s0) & 1u) * p.tile_bytes + BR_SLAB * p.k_pitch + half * KEYS * p.v_pitch;
+            const float *ks = s_scales[(slab - s0) & 3u][0] + half * KEYS, *vs = s_scales[(slab - s0) & 3u][1] + half * KEYS;
+            float s[4][4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) s[j][x] = 0.0f;
+            // the operands of a step are requested while the products of the step before run
+            const uint32_t q_from = q_at + (rows16 * 16 + (lane & 15u)) * p.q_pitch + 16 * (lane >> 4), k_from = k_at + (8 * (lane >> 4) + (lane & 7u)) * p.k_pitch + 16 * ((lane >> 3) & 1u);
+            uint32_t q[2][4], q2[2][4], w[2][2][4];
+            auto fetch = [&](int k) {
+                ldsm4(q_from + 32 * k, q[k & 1]);
+                if (TWO) ldsm4(q_from + BR_ROWS * p.q_pitch + 32 * k, q2[k & 1]);
+                ldsm4(k_from + 32 * k, w[k & 1][0]);
+                ldsm4(k_from + 16 * p.k_pitch + 32 * k, w[k & 1][1]);
+            };
+            fetch(0);
 #pragma unroll
             for (int k = 0; k < KSTEPS; ++k) {
                 if (16 * k >= dim) break;
-                uint32_t q[4], q2[4];
-                ldsm4(q_at + (warp * 16 + (lane & 15u)) * p.q_pitch + 32 * k + 16 * (lane >> 4), q);
-                if (TWO) ldsm4(q_at + (BR_ROWS + warp * 16 + (lane & 15u)) * p.q_pitch + 32 * k + 16 * (lane >> 4), q2);
+                if (k + 1 < KSTEPS && 16 * (k + 1) < dim) fetch(k + 1);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t w[4];
-                    ldsm4(k_at + (16 * j + 8 * (lane >> 4) + (lane & 7u)) * p.k_pitch + 32 * k + 16 * ((lane >> 3) & 1u), w);
-                    mma_f16(s[2 * j], q, w[0], w[1]);
-                    mma_f16(s[2 * j + 1], q, w[2], w[3]);
-                    if (TWO) {
-                        mma_f16(s[2 * j], q2, w[0], w[1]);
-                        mma_f16(s[2 * j + 1], q2, w[2], w[3]);
-                    }
+                for (int j = 0; j < 2; ++j) {
+                    mma_f16(s[2 * j], q[k & 1], w[k & 1][j][0], w[k & 1][j][1]);
+                    mma_f16(s[2 * j + 1], q[k & 1], w[k & 1][j][2], w[k & 1][j][3]);
                 }
-            }
-            const uint32_t key0 = slab * BR_SLAB + 2 * in_quad;
+                if (TWO)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+                    for (int j = 0; j < 2; ++j) {
+                        mma_f16(s[2 * j], q2[k & 1], w[k & 1][j][0], w[k & 1][j][1]);
+                        mma_f16(s[2 * j + 1], q2[k & 1], w[k & 1][j][2], w[k & 1][j][3]);
+                    }
+            }
+            const uint32_t key0 = slab * BR_SLAB + half * KEYS + 2 * in_quad;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
                 const float2 f = *reinterpret_cast<const float2*>(ks + 8 * j + 2 * in_quad);
                 s[j][0] *= row_scale[0] * f.x; s[j][1] *= row_scale[0] * f.y;
                 s[j][2] *= row_scale[1] * f.x; s[j][3] *= row_scale[1] * f.y;
             }
-            if ((slab + 1) * BR_SLAB > common) {
+            if (slab * BR_SLAB + half * KEYS + KEYS > common) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
                         if (key0 + 8 * j + (x & 1) >= limit[x >> 1]) s[j][x] = -INFINITY;
             }
             float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 most[0] = fmaxf(most[0], fmaxf(s[j][0], s[j][1]));
                 most[1] = fmaxf(most[1], fmaxf(s[j][2], s[j][3]));
             }
@@ -234,12 +244,8 @@ block_rows_kernel(const __grid_constant__ BlockRowsParams p) {
                 most[x] = fmaxf(most[x], __shfl_xor_sync(0xffffffffu, most[x], 1));
                 most[x] = fmaxf(most[x], __shfl_xor_sync(0xffffffffu, most[x], 2));
             }
-            int e = -110;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const float largest = vs[lane + 32 * x];
-                if (largest > 0.0f && largest < INFINITY) e = max(e, (int)(__float_as_uint(largest) >> 23) - 126);
-            }
+            const float largest = vs[lane];
+            int e = largest > 0.0f && largest < INFINITY ? max((int)(__float_as_uint(largest) >> 23) - 126, -110) : -110;
             e = __reduce_max_sync(0xffffffffu, e);
             if (__any_sync(0xffffffffu, most[0] > top[0] || most[1] > top[1]) || e > lift) {
                 const int higher = max(e, lift);
@@ -263,36 +269,83 @@ block_rows_kernel(const __grid_constant__ BlockRowsParams p) {
                     }
             }
             const float t0 = top[0] == -INFINITY ? 0.0f : top[0], t1 = top[1] == -INFINITY ? 0.0f : top[1], raise = power_of_two(min(14 - lift, 127));
+            uint32_t u[2][4], u2[2][4];
 #pragma unroll
-            for (int t = 0; t < BR_SLAB / 16; ++t) {
-                uint32_t w[4], w2[4];
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = *reinterpret_cast<const float2*>(vs + 8 * j + 2 * in_quad);
+                const float e0 = ex2(s[j][0] - t0), e1 = ex2(s[j][1] - t0), e2 = ex2(s[j][2] - t1), e3 = ex2(s[j][3] - t1);
+                sum[0] += e0 + e1;
+                sum[1] += e2 + e3;
+                const float f0 = f.x * raise, f1 = f.y * raise, y0 = e0 * f0, y1 = e1 * f1, y2 = e2 * f0, y3 = e3 * f1;
+                u[j >> 1][2 * (j & 1)] = half_pair(y0, y1);
+                u[j >> 1][2 * (j & 1) + 1] = half_pair(y2, y3);
+                if (TWO) {
+                    const float2 h0 = half_values(u[j >> 1][2 * (j & 1)]), h1 = half_values(u[j >> 1][2 * (j & 1) + 1]);
+                    u2[j >> 1][2 * (j & 1)] = half_pair(y0 - h0.x, y1 - h0.y);
+                    u2[j >> 1][2 * (j & 1) + 1] = half_pair(y2 - h1.x, y3 - h1.y);
+                }
+            }
+            const uint32_t v_from = v_at + (lane & 15u) * p.v_pitch + 16 * (lane >> 4);
+            uint32_t v[2][2][4];
+            auto fetch_v = [&](int i) {
+                ldsm4t(v_from + 32 * i, v[i & 1][0]);
+                ldsm4t(v_from + 16 * p.v_pitch + 32 * i, v[i & 1][1]);
+            };
+            fetch_v(0);
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const int j = 2 * t + y;
-                    const float2 f = *reinterpret_cast<const float2*>(vs + 8 * j + 2 * in_quad);
-                    const float e0 = ex2(s[j][0] - t0), e1 = ex2(s[j][1] - t0), e2 = ex2(s[j][2] - t1), e3 = ex2(s[j][3] - t1);
-                    sum[0] += e0 + e1;
-                    sum[1] += e2 + e3;
-                    const float f0 = f.x * raise, f1 = f.y * raise, y0 = e0 * f0, y1 = e1 * f1, y2 = e2 * f0, y3 = e3 * f1;
-                    w[2 * y] = half_pair(y0, y1);
-                    w[2 * y + 1] = half_pair(y2, y3);
+            for (int i = 0; i < CHUNKS; ++i) {
+                if (16 * i >= vdim) break;
+                if (i + 1 < CHUNKS && 16 * (i + 1) < vdim) fetch_v(i + 1);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    mma_f16(o[i][0], u[t], v[i & 1][t][0], v[i & 1][t][1]);
+                    mma_f16(o[i][1], u[t], v[i & 1][t][2], v[i & 1][t][3]);
                     if (TWO) {
-                        const float2 h0 = half_values(w[2 * y]), h1 = half_values(w[2 * y + 1]);
-                        w2[2 * y] = half_pair(y0 - h0.x, y1 - h0.y);
-                        w2[2 * y + 1] = half_pair(y2 - h1.x, y3 - h1.y);
+                        mma_f16(o[i][0], u2[t], v[i & 1][t][0], v[i & 1][t][1]);
+                        mma_f16(o[i][1], u2[t], v[i & 1][t][2], v[i & 1][t][3]);
                     }
                 }
+            }
+        }
+        // ---- the second half's results join the first's, through the memory of queries and tiles ----
+        const float back = lift == -1000 ? 0.0f : power_of_two(lift - 14);
 #pragma unroll
-                for (int i = 0; i < CHUNKS; ++i) {
-                    if (16 * i >= vdim) break;
-                    uint32_t v[4];
-                    ldsm4t(v_at + (16 * t + (lane & 15u)) * p.v_pitch + 32 * i + 16 * (lane >> 4), v);
-                    mma_f16(o[i][0], w, v[0], v[1]);
-                    mma_f16(o[i][1], w, v[2], v[3]);
-                    if (TWO) {
-                        mma_f16(o[i][0], w2, v[0], v[1]);
-                        mma_f16(o[i][1], w2, v[2], v[3]);
-                    }
+        for (int x = 0; x < 2; ++x) {
+            sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 1);
+            sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 2);
+        }
+        float* s_o = reinterpret_cast<float*>(smem);       // [128][vdim + 2]
+        __syncthreads();        // queries and tiles have been read
+        if (half && works) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                float* to = s_o + (rows16 * 16 + quad + 8 * x) * (vdim + 2);
+#pragma unroll
+                for (int i = 0; i < 2 * CHUNKS; ++i) {
+                    if (8 * i >= vdim) break;
+                    *reinterpret_cast<float2*>(to + 8 * i + 2 * in_quad) = make_float2(o[i >> 1][i & 1][2 * x] * back, o[i >> 1][i & 1][2 * x + 1] * back);
+                }
+                if (in_quad == 0) *reinterpret_cast<float2*>(to + vdim) = make_float2(top[x], sum[x]);
+            }
+        }
+        __syncthreads();
+        if (!half && works) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const float* add = s_o + (rows16 * 16 + quad + 8 * x) * (vdim + 2);
+                const float2 ml = *reinterpret_cast<const float2*>(add + vdim);
+                const float t = fmaxf(top[x], ml.x);
+                // a half that saw nothing has no sum; NaN is not 0
+                const float f = sum[x] == 0.0f ? 0.0f : ex2(top[x] - t), g = ml.y == 0.0f ? 0.0f : ex2(ml.x - t);
+                sum[x] = fmaf(f, sum[x], g * ml.y);
+                top[x] = t;
+#pragma unroll
+                for (int i = 0; i < 2 * CHUNKS; ++i) {
+                    if (8 * i >= vdim) break;
+                    const float2 y = *reinterpret_cast<const float2*>(add + 8 * i + 2 * in_quad);
+                    float &lo = o[i >> 1][i & 1][2 * x], &hi = o[i >> 1][i & 1][2 * x + 1];
+                    lo = fmaf(f * back, lo, g * y.x);
+                    hi = fmaf(f * back, hi, g * y.y);
                 }
             }
         }
@@ -303,28 +356,34 @@ block_rows_kernel(const __grid_constant__ BlockRowsParams p) {
             const uint32_t flat = at.tile * BR_ROWS + r;
             return (uint64_t)(at.first_row + flat / group) * a.ld + (uint64_t)(at.head * group + flat % group) * vdim;
         };
-        const float back = lift == -1000 ? 0.0f : power_of_two(lift - 14);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const uint32_t r = warp * 16 + quad + 8 * x;
-            sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 1);
-            sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 2);
-            if (r >= rows) continue;
-            const float by = whole ? sum[x] == 0.0f ? 0.0f : __fdiv_rn(back, sum[x]) : back;
-            const uint64_t out = out_of(r);
-#pragma unroll
-            for (int i = 0; i < 2 * CHUNKS; ++i) {
-                if (8 * i >= vdim) break;
-                const float lo = o[i >> 1][i & 1][2 * x] * by, hi = o[i >> 1][i & 1][2 * x + 1] * by;
-                const uint32_t col = 8 * i + 2 * in_quad;
-                if (whole) {
-                    seq_store(a.out, out + col, lo, a.dtype);
-                    seq_store(a.out, out + col + 1, hi, a.dtype);
-                } else {
-                    __stcg(reinterpret_cast<float2*>(partial + r * (vdim + 2) + col), make_float2(lo, hi));
-                }
+        const bool pairs_ok = ((uintptr_t)a.out % 8u) == 0 && a.ld % 2 == 0;      // two values a store
+        auto store2 = [&](uint64_t i, float lo, float hi) {
+            if (!pairs_ok) {
+                seq_store(a.out, i, lo, a.dtype);
+                seq_store(a.out, i + 1, hi, a.dtype);
+            } else if (a.dtype == HOLO_DTYPE_F32) {
+                *reinterpret_cast<float2*>((float*)a.out + i) = make_float2(lo, hi);
+            } else {
+                *reinterpret_cast<uint32_t*>((uint16_t*)a.out + i) = a.dtype == HOLO_DTYPE_F16 ? half_pair(lo, hi) : pack_bf16(lo, hi);
             }
-            if (!whole && in_quad == 0) __stcg(reinterpret_cast<float2*>(partial + r * (vdim + 2) + vdim), make_float2(top[x], sum[x]));
+        };
+        if (!half && works) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t r = rows16 * 16 + quad + 8 * x;
+                if (r >= rows) continue;
+                const float by = whole ? sum[x] == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum[x]) : 1.0f;
+                const uint64_t out = out_of(r);
+#pragma unroll
+                for (int i = 0; i < 2 * CHUNKS; ++i) {
+                    if (8 * i >= vdim) break;
+                    const float lo = o[i >> 1][i & 1][2 * x] * by, hi = o[i >> 1][i & 1][2 * x + 1] * by;
+                    const uint32_t col = 8 * i + 2 * in_quad;
+                    if (whole) store2(out + col, lo, hi);
+                    else __stcg(reinterpret_cast<float2*>(partial + r * (vdim + 2) + col), make_float2(lo, hi));
+                }
+                if (!whole && in_quad == 0) __stcg(reinterpret_cast<float2*>(partial + r * (vdim + 2) + vdim), make_float2(top[x], sum[x]));
+            }
         }
         if (!whole) {
             // the plane's CTAs, and its counter: that of the CTA it begins in
@@ -365,8 +424,7 @@ block_rows_kernel(const __grid_constant__ BlockRowsParams p) {
                         v = make_float2(fmaf(f, y.x, v.x), fmaf(f, y.y, v.y));
                     }
                     const uint64_t out = out_of(r);
-                    seq_store(a.out, out + col, v.x, a.dtype);
-                    seq_store(a.out, out + col + 1, v.y, a.dtype);
+                    store2(out + col, v.x, v.y);
                 }
             }
         }
@@ -391,6 +449,7 @@ int32_t launch_block_rows(holo_b200_ctx* ctx, BlockRowsParams& p) {
     uint32_t smem = p.q_bytes + 2 * p.tile_bytes + BR_STAGES * p.stage_bytes;
     const uint32_t weights = BR_ROWS * 4 * (uint32_t)ctx->sm_count;       // of a plane's parts
     if (smem < weights) smem = weights;
+    if (smem < BR_ROWS * (vdim + 2) * 4) smem = BR_ROWS * (vdim + 2) * 4;       // a half's results
     if (smem > (uint32_t)ctx->smem_optin - 4096) return holo_fail(HOLO_ERR_DISPATCH, "dispatch failed: block_cache_attention needs %u bytes of shared memory", smem);
     static thread_local int configured_device = -1;
     if (configured_device != ctx->device) {
