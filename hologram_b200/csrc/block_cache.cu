@@ -287,6 +287,8 @@ int32_t holo_launch_block_cache_write(holo_b200_ctx* ctx, const HoloBlockWriteAr
 
 int32_t holo_launch_block_cache_attention(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a) {
     bool taken;
+    HOLO_TRY(holo_try_block_tile(ctx, a, &taken));
+    if (taken) return HOLO_OK;
     HOLO_TRY(holo_try_block_rows(ctx, a, &taken));
     if (taken) return HOLO_OK;
     HOLO_TRY(holo_try_block_attention(ctx, a, &taken));

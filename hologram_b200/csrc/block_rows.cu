@@ -463,6 +463,18 @@ int32_t launch_block_rows(holo_b200_ctx* ctx, BlockRowsParams& p) {
 
 }  // namespace
 
+// The buffer of partial results, from the first call on
+int32_t holo_block_row_partials(holo_b200_ctx* ctx) {
+    if (!ctx->block_row_partials) {
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        HOLO_CUDA(cudaStreamIsCapturing(ctx->stream, &capturing));
+        if (capturing != cudaStreamCaptureStatusNone)
+            return holo_fail(HOLO_ERR_DISPATCH, "dispatch failed: block_cache_attention allocates its buffer on its first call, which cannot be recorded: make one before");
+        HOLO_CUDA(cudaMalloc(&ctx->block_row_partials, (uint64_t)ctx->sm_count * 2 * BR_ROWS * (128 + 2) * sizeof(float)));
+    }
+    return HOLO_OK;
+}
+
 int32_t holo_try_block_rows(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool* taken) {
     *taken = false;
     const HoloBlockCache& c = a.c;
@@ -473,13 +485,7 @@ int32_t holo_try_block_rows(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool
     // slabs of the whole list of 32 bits
     const uint64_t tiles = ((uint64_t)c.rows * group / BR_ROWS + c.sequences) * c.kv_heads;
     if ((uint64_t)c.rows * a.heads > 0x7fffffffull || tiles > 0x7fffffffull / (((uint64_t)c.table_ld * c.block_rows + BR_SLAB - 1) / BR_SLAB)) return HOLO_OK;
-    if (!ctx->block_row_partials) {
-        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-        HOLO_CUDA(cudaStreamIsCapturing(ctx->stream, &capturing));
-        if (capturing != cudaStreamCaptureStatusNone)
-            return holo_fail(HOLO_ERR_DISPATCH, "dispatch failed: block_cache_attention allocates its buffer on its first call, which cannot be recorded: make one before");
-        HOLO_CUDA(cudaMalloc(&ctx->block_row_partials, (uint64_t)ctx->sm_count * 2 * BR_ROWS * (128 + 2) * sizeof(float)));
-    }
+    HOLO_TRY(holo_block_row_partials(ctx));
     *taken = true;
     BlockRowsParams p = {};
     p.a = a;

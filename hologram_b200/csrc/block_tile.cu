@@ -1,0 +1,550 @@
+// Attention of many rows of each sequence (portions of prompts) over the int8 block cache on tcgen05, for 16-bit queries, dims in steps of
+// 16 up to 128 and blocks of a multiple of 16 rows.
+//
+// A CTA takes 128 query rows of a kv head (a row is a new position and a head of the group) and walks the keys in tiles of 128:
+//   warps 8-11 turn the tiles' codes into f16 (exact: integers of 8 bits) in the operands' swizzled layout, K and V through rings of two, a
+//              tile's codes on their way in registers while the one before is turned; and the query rows, scaled by a power of two to a largest
+//              value in [2^14, 2^15): exact in f16 but for values 2^29 smaller than the largest
+//   warp 1     tcgen05.mma issuer: S = Q K^T, then O += P V with P read from TMEM
+//   warps 4-7  softmax, one thread per row. A block's scales are the same for 16 keys in a row: the key scale is a factor of the scores, the
+//              value scale a term of the exponent, w = 2^(s - max + log2 scale_v), and is taken out of the row's sum again. Weights are
+//              relative to a power of two above the largest value scale of the CTA's keys and rounded to f16 (2^-12 of a weight)
+// The tiles of all planes form one list that the CTAs share out evenly; parts of a plane are joined as for few rows (block_list.cuh).
+// Bound: one tile's chain scores -> softmax -> product; 128 rows leave the tensor core idle meanwhile. TMEM: S at 0, its weights over it, O at 128.
+#include "attention_issue.cuh"
+#include "block_list.cuh"
+
+namespace {
+
+constexpr int BT_ROWS = 128, BT_TILE = 128, BT_WARPS = 12, BT_WORKERS = 128;      // threads that turn codes
+constexpr float BT_GROWTH = 8.0f;
+constexpr int BT_LIFT = 7;
+
+struct BlockTileParams {
+    HoloBlockAttnArgs a;
+    float* partials;          // [CTAs][2][128 rows][vdim + 2]
+    uint32_t* arrivals;       // a counter per CTA, zero between launches
+    uint32_t group, k_chunks, v_chunks;      // chunks of 64 columns
+    int32_t br_shift;
+};
+
+constexpr uint32_t PICK01 = 0x4140, PICK23 = 0x4342;
+
+// UNITS: 16-byte units of codes of a row, at most; a worker thread has one key and all its units
+template <int UNITS>
+__global__ void __launch_bounds__(BT_WARPS * 32, 1)
+block_tile_kernel(const __grid_constant__ BlockTileParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    const HoloBlockAttnArgs& a = p.a;
+    const HoloBlockCache& c = a.c;
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t* sm = smem_raw + (base - raw);
+    const uint32_t k_bytes = p.k_chunks * TILE_CHUNK, v_bytes = p.v_chunks * TILE_CHUNK;
+    const uint32_t o_k = k_bytes, o_v = o_k + 2 * k_bytes, o_bars = o_v + 2 * v_bytes, bars = base + o_bars;
+    const uint32_t bar_q_full = bars, bar_q_empty = bars + 8, bar_k_full = bars + 16, bar_k_empty = bars + 32, bar_v_full = bars + 48, bar_v_empty = bars + 64,
+                   bar_s = bars + 80, bar_pa = bars + 88, bar_pb = bars + 96, bar_pv = bars + 104;
+    uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sm + o_bars + 120);
+    volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(sm + o_bars + 124);
+    uint32_t* s_last = reinterpret_cast<uint32_t*>(sm + o_bars + 128);
+    int* s_lift = reinterpret_cast<int*>(sm + o_bars + 132);                       // [2], by plane
+    uint32_t* s_most = reinterpret_cast<uint32_t*>(sm + o_bars + 144);              // [2][4], by plane
+    const uint32_t bar_workers = bars + 176, bar_rows = bars + 184;                  // the four worker warps meet, the four softmax warps
+    float* s_row = reinterpret_cast<float*>(sm + o_bars + 256);                     // [2][128], by plane
+    float* s_scale = s_row + 2 * BT_ROWS;                                           // [4][3][8], by tile: key scales; exponents; reciprocals
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = p.group, dim = c.dim, vdim = c.vdim, br = c.block_rows;
+    if (tid == 0) {
+        mbar_init(bar_q_full, 4);             // one arrival per worker warp
+        mbar_init(bar_q_empty, 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(bar_k_full + 8 * s, 4);
+            mbar_init(bar_k_empty + 8 * s, 1);
+            mbar_init(bar_v_full + 8 * s, 4);
+            mbar_init(bar_v_empty + 8 * s, 1);
+        }
+        mbar_init(bar_s, 2);                  // the scores, and the issuer that has seen the tile's scales
+        mbar_init(bar_workers, 4);
+        mbar_init(bar_rows, 4);
+        mbar_init(bar_pa, 4);                 // one arrival per softmax warp
+        mbar_init(bar_pb, 4);
+        mbar_init(bar_pv, 1);
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    holo_pdl_wait();
+    if (blockIdx.x == 0) check_sequences(c.starts, c.lengths, c.sequences, c.rows, (int64_t)c.table_ld * br, c.status);
+    Share mine;
+    if (!find_share<BT_ROWS, BT_TILE, 2, 4>(c, group, &mine)) return;       // the same for every thread
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(256u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    holo_pdl_trigger();
+    const uint32_t tmem_base = *s_tmem;
+    // everybody walks the planes by itself
+    auto keys_of = [&](const Plane& f) { return (uint32_t)f.length - (f.n - rows_before<BT_ROWS>(f, f.tile, group)); };
+    auto more = [&](Plane& f) {
+        if (f.at + f.slabs >= mine.hi) return false;
+        next_plane<BT_ROWS, BT_TILE>(c, group, &f);
+        return f.slabs != 0;
+    };
+
+    auto arrive_at = [&](uint32_t bar) {
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+    };
+    auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, long_wait(bar, parity, s_abort, c.status)) != 0; };
+
+    if (warp >= 8) {
+        // ---------------- workers: codes and queries into operands ----------------
+        const uint32_t me = tid - 8 * 32;
+        uint32_t nt = 0, np = 0;
+        bool ok = true;
+        auto block_of = [&](uint32_t pos) { return p.br_shift >= 0 ? pos >> p.br_shift : pos / br; };
+        // 16 codes as 32 bytes of a 128-byte row: the row's 16-byte units stand at their number xor key % 8
+        auto turn = [&](uint8_t* tile, uint32_t unit, const uint4& v) {
+            const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
+            uint32_t h[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                h[2 * e] = codes_to_half<PICK01>(w[e]);
+                h[2 * e + 1] = codes_to_half<PICK23>(w[e]);
+            }
+            uint4* to = reinterpret_cast<uint4*>(tile + (unit >> 2) * TILE_CHUNK + me * 128);
+            to[(2 * (unit & 3u)) ^ (me & 7u)] = make_uint4(h[0], h[1], h[2], h[3]);
+            to[(2 * (unit & 3u) + 1) ^ (me & 7u)] = make_uint4(h[4], h[5], h[6], h[7]);
+        };
+        auto arrive = [&](uint32_t bar) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive_at(bar);
+        };
+        Plane at = mine.first;
+        do {
+            uint32_t s0, s1;
+            mine.ends_of(at, &s0, &s1);
+            const uint32_t sees = keys_of(at), rows = min((uint32_t)BT_ROWS, at.n * group - at.tile * BT_ROWS);
+            // the block that holds this thread's key of a tile, or -1
+            auto find = [&](uint32_t tile) {
+                const uint32_t pos = tile * BT_TILE + me;
+                if (tile >= s1 || pos >= sees) return -1;
+                const int id = c.table[(uint64_t)at.seq * c.table_ld + block_of(pos)];
+                if ((uint32_t)id < c.blocks) return id;
+                atomicOr(c.status, HOLO_STATUS_TABLE);
+                return -1;
+            };
+            int id = find(s0), next_id = find(s0 + 1);
+            uint4 kreg[UNITS], vreg[UNITS];
+            float ks = 0.0f, vs = 0.0f;
+            auto row_of = [&](uint32_t tile, int b) {
+                const uint32_t pos = tile * BT_TILE + me;
+                return ((uint64_t)(uint32_t)b * c.kv_heads + at.head) * br + (pos - block_of(pos) * br);
+            };
+            auto load_k = [&](uint32_t tile, int b) {
+                const uint4* from = reinterpret_cast<const uint4*>(c.k_codes + (b < 0 ? 0 : row_of(tile, b) * dim));
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u) kreg[u] = b >= 0 && 16 * u < dim ? from[u] : make_uint4(0, 0, 0, 0);
+                const uint64_t plane = (uint64_t)(uint32_t)max(b, 0) * c.kv_heads + at.head;
+                ks = b < 0 ? 0.0f : c.k_scales[plane];
+                vs = b < 0 ? 0.0f : c.v_scales[plane];
+            };
+            auto load_v = [&](uint32_t tile, int b) {
+                const uint4* from = reinterpret_cast<const uint4*>(c.v_codes + (b < 0 ? 0 : row_of(tile, b) * vdim));
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u) vreg[u] = b >= 0 && 16 * u < vdim ? from[u] : make_uint4(0, 0, 0, 0);
+            };
+            load_k(s0, id);
+            load_v(s0, id);
+            // the largest value scale of the CTA's part of the plane
+            float largest = 0.0f;
+            for (uint32_t b = block_of(s0 * BT_TILE) + me, last = block_of(min(s1 * BT_TILE, sees) - 1); b <= last; b += BT_WORKERS) {
+                const int x = c.table[(uint64_t)at.seq * c.table_ld + b];
+                const float f = (uint32_t)x < c.blocks ? c.v_scales[(uint64_t)x * c.kv_heads + at.head] : 0.0f;
+                if (f < INFINITY) largest = fmaxf(largest, f);
+            }
+            const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
+            volatile uint32_t* most_of = s_most + 4 * (np & 1u);
+            if (lane == 0) most_of[warp - 8] = bits;
+            arrive_at(bar_workers);
+            // the queries' memory is free when the last plane's last scores are there
+            ok = (np == 0 || all_wait(bar_q_empty, (np - 1) & 1u)) && all_wait(bar_workers, np & 1u);
+            if (!ok) break;
+            const uint32_t top_bits = max(max(most_of[0], most_of[1]), max(most_of[2], most_of[3]));
+            const int lift = max((int)(top_bits >> 23) - 126, -100);       // 2^lift is above it
+            if (me == 0) s_lift[np & 1u] = lift;
+            // query rows, a warp a row at a time: all lanes a row's columns
+            const uint32_t halves = dim / 2;
+#pragma unroll 4
+            for (uint32_t r = (warp - 8) * 32; r < (warp - 8) * 32 + 32; ++r) {
+                const uint32_t flat = at.tile * BT_ROWS + r, i = flat / group, head = at.head * group + flat % group;
+                float2 x[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                float most = 0.0f;
+                bool finite = true;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t d = lane + 32 * e;
+                    if (r < rows && d < halves) {
+                        const uint64_t q = (uint64_t)(at.first_row + i) * a.q_ld + (uint64_t)head * dim + 2 * d;
+                        x[e] = make_float2(seq_load(a.q, q, a.dtype), seq_load(a.q, q + 1, a.dtype));
+                    }
+                    most = fmaxf(most, fmaxf(fabsf(x[e].x), fabsf(x[e].y)));
+                    finite = finite && fabsf(x[e].x) < INFINITY && fabsf(x[e].y) < INFINITY;
+                }
+                const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+                finite = __all_sync(0xffffffffu, finite);
+                // 2^e <= most < 2^(e + 1); two factors, since 2^(14 - e) alone may overflow
+                const int up = finite && m ? 14 - (m >> 23 ? (int)(m >> 23) - 127 : -118 - __clz((int)m)) : 0;
+                const float f0 = power_of_two(up / 2), f1 = power_of_two(up - up / 2);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t d = lane + 32 * e;       // pair of columns: 32 pairs are a chunk of 64 columns, 4 pairs a unit
+                    if (d < halves)
+                        *reinterpret_cast<uint32_t*>(sm + e * TILE_CHUNK + r * 128 + (((lane >> 2) ^ (r & 7u)) << 4) + 4 * (lane & 3u)) =
+                            finite ? half_pair(x[e].x * f0 * f1, x[e].y * f0 * f1) : 0u;
+                }
+                if (lane == 0) s_row[(np & 1u) * BT_ROWS + r] = finite ? a.scale * LOG2E * power_of_two(-(up / 2)) * power_of_two(-(up - up / 2)) : NAN;
+            }
+            arrive(bar_q_full);
+            ++np;
+#pragma unroll 1
+            for (uint32_t t = s0; t < s1 && ok; ++t, ++nt) {
+                const uint32_t stage = nt & 1u;
+                // scales of 16 keys in a row, from the thread that has the first of them. A value scale 2^-60 of the largest and less is as good
+                // as none; its keys' weights still count in the rows' sums
+                if ((me & 15u) == 0) {
+                    float* to = s_scale + (nt & 3u) * 24 + (me >> 4);
+                    const float x = fmaxf(vs, power_of_two(max(lift - 60, -126)));
+                    to[0] = ks;
+                    to[8] = __log2f(x) + (float)(BT_LIFT - lift);
+                    to[16] = __fdiv_rn(1.0f, x) * power_of_two(lift - BT_LIFT);
+                }
+                ok = nt < 2 || all_wait(bar_k_empty + 8 * stage, ((nt >> 1) - 1) & 1u);
+                if (!ok) break;
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u)
+                    if (16 * u < dim) turn(sm + o_k + stage * k_bytes, u, kreg[u]);
+                arrive(bar_k_full + 8 * stage);
+                const int after = find(t + 2);
+                load_k(t + 1, next_id);
+                ok = nt < 2 || all_wait(bar_v_empty + 8 * stage, ((nt >> 1) - 1) & 1u);
+                if (!ok) break;
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u)
+                    if (16 * u < vdim) turn(sm + o_v + stage * v_bytes, u, vreg[u]);
+                arrive(bar_v_full + 8 * stage);
+                load_v(t + 1, next_id);
+                next_id = after;
+            }
+        } while (ok && more(at));
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        const uint32_t elected = lane == 0;
+        // D = f32, A and B f16, M = 128; S: both operands K-major, N = 128; O: V is N-major, N = vdim
+        const uint32_t idesc_s = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+        const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((vdim >> 3) << 17) | ((128u >> 4) << 24);
+        const uint64_t first_q = smem_desc(uniform(base), 16, 1024), first_v = smem_desc(uniform(base + o_v), TILE_CHUNK, 1024);
+        const uint32_t desc_q = (uint32_t)first_q, desc_k = (uint32_t)smem_desc(uniform(base + o_k), 16, 1024), high_s = (uint32_t)(first_q >> 32);
+        const uint32_t desc_v = (uint32_t)first_v, high_v = (uint32_t)(first_v >> 32), tmem_s = uniform(tmem_base), tmem_o = tmem_s + 128, ub = uniform(bars);
+        const uint32_t ksteps = dim / 16;
+        uint32_t nk = 0, nv = 0, np = 0;
+        bool ok = true;
+        auto wait = all_wait;
+        Plane at = mine.first;
+        do {
+            uint32_t s0, s1;
+            mine.ends_of(at, &s0, &s1);
+            const uint32_t tiles = uniform(s1 - s0), keys = uniform(keys_of(at) - s0 * BT_TILE);
+            ok = wait(bar_q_full, np & 1u);
+            ++np;
+            for (uint32_t t = 0; t <= tiles && ok; ++t) {
+                // the product of key tile t - 1, the scores of key tile t
+                if (t < tiles) ok = wait(bar_k_full + 8 * (nk & 1u), (nk >> 1) & 1u);
+                if (ok && t > 0) {
+                    const uint32_t dv = desc_v + (nv & 1u) * (v_bytes >> 4), steps = min(8u, (keys - (t - 1) * 128 + 15) / 16);
+                    ok = wait(bar_v_full + 8 * (nv & 1u), (nv >> 1) & 1u) && wait(bar_pa, nv & 1u);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) elected_ts(elected & (uint32_t)(k < steps), tmem_o, tmem_s + k * 8, dv + 128 * k, high_v, idesc_o, k | (t > 1));
+                    ok = wait(bar_pb, nv & 1u);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                    for (uint32_t k = 4; k < 8; ++k) elected_ts(elected & (uint32_t)(k < steps), tmem_o, tmem_s + k * 8, dv + 128 * k, high_v, idesc_o, 1);
+                    if (t == tiles) elected_commit(elected, ub + 104);
+                }
+                if (ok && t < tiles) {
+                    // the next scores go where the weights are, behind the product that reads them (see product_ss)
+                    const uint32_t dk = desc_k + (nk & 1u) * (k_bytes >> 4);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; ++k) {
+                        const uint32_t off = (k >> 2) * (TILE_CHUNK >> 4) + 2 * (k & 3u);
+                        elected_ss(elected & (uint32_t)(k < ksteps), tmem_s, desc_q + off, high_s, dk + off, high_s, idesc_s, k != 0);
+                    }
+                    elected_commit(elected, ub + 80);
+                    arrive_at(ub + 80);
+                }
+                if (!ok) break;
+                if (t > 0) {
+                    elected_commit(elected, ub + 64 + 8 * (nv & 1u));
+                    ++nv;
+                }
+                if (t < tiles) {
+                    elected_commit(elected, ub + 32 + 8 * (nk & 1u));
+                    ++nk;
+                    if (t + 1 == tiles) elected_commit(elected, ub + 8);
+                }
+            }
+        } while (ok && more(at));
+    } else if (warp >= 4) {
+        // ---------------- softmax (TMEM lane quarter = warp % 4), then the output ----------------
+        const uint32_t quarter = warp & 3u, lanes = (quarter * 32u) << 16, r = quarter * 32 + lane;
+        const uint32_t tmem_s = tmem_base + lanes, tmem_o = tmem_base + 128 + lanes;
+        uint32_t nt = 0, np = 0, met = 0;
+        bool ok = true;
+        Plane at = mine.first;
+        do {
+            uint32_t s0, s1;
+            mine.ends_of(at, &s0, &s1);
+            const uint32_t rows = min((uint32_t)BT_ROWS, at.n * group - at.tile * BT_ROWS);
+            const uint32_t i = (at.tile * BT_ROWS + min(r, rows - 1)) / group, limit = (uint32_t)max(0, at.length - (int32_t)(at.n - i - 1));
+            const uint32_t common = __reduce_min_sync(0xffffffffu, limit);
+            // (the queries' barrier may be a plane ahead of this warp: what the workers left for the plane is read behind its first scores)
+            float top = -INFINITY, sum = 0.0f, row_scale = 0.0f, back = 0.0f;
+            for (uint32_t t = s0; t < s1; ++t, ++nt) {
+                ok = all_wait(bar_s, nt & 1u);
+                if (!ok) break;
+                if (t == s0) {
+                    row_scale = s_row[(np & 1u) * BT_ROWS + r];
+                    back = power_of_two(s_lift[np & 1u] - BT_LIFT);
+                    if (row_scale != row_scale) sum = NAN;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t v[4][32];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) tmem_ld32_request(tmem_s + 32 * x, v[x]);
+                const float* scale = s_scale + (nt & 3u) * 24;
+                auto factor = [&](int g) { return fmaxf(row_scale * scale[g], 1e-37f); };      // above 0: -inf stays -inf
+                tmem_ld32_wait(v[0]);
+#pragma unroll
+                for (int x = 1; x < 4; ++x) tmem_ld32_pass(v[x]);
+                const uint32_t key0 = t * BT_TILE;
+                if (key0 + 128 > common) {
+                    const uint32_t hi = limit > key0 ? limit - key0 : 0u;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const uint32_t seen = hi <= 32u * x ? 0u : hi >= 32u * x + 32 ? 0xffffffffu : (1u << (hi - 32u * x)) - 1u;
+#pragma unroll
+                        for (int y = 0; y < 32; ++y)
+                            if (!(seen >> y & 1u)) v[x][y] = 0xff800000u;
+                    }
+                }
+                float here = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    float m = -INFINITY;
+#pragma unroll
+                    for (int y = 0; y < 16; y += 2) m = fmaxf(fmaxf(m, __uint_as_float(v[g >> 1][16 * (g & 1) + y])), __uint_as_float(v[g >> 1][16 * (g & 1) + y + 1]));
+                    here = fmaxf(here, m * factor(g));
+                }
+                const bool grows = here > top + BT_GROWTH;
+                if (__any_sync(0xffffffffu, grows)) {
+                    const float f = grows ? ex2(top - here) : 1.0f;      // 0 from the first scores on
+                    if (grows) top = here;
+                    sum *= f;
+                    if (t > s0) {    // the barrier of this tile's scores stands for the product before them too: O is at rest
+                        const uint64_t f2 = pair(f, f);
+                        for (uint32_t x = 0; x < vdim; x += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(tmem_o + x, o);
+#pragma unroll
+                            for (int y = 0; y < 8; ++y) {
+                                const float2 m = unpair(mul2(pair(__uint_as_float(o[2 * y]), __uint_as_float(o[2 * y + 1])), f2));
+                                o[2 * y] = __float_as_uint(m.x);
+                                o[2 * y + 1] = __float_as_uint(m.y);
+                            }
+                            tmem_st16(tmem_o + x, o);
+                        }
+                    }
+                }
+                const float less = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int g = 2 * x + h;
+                        const float term = scale[8 + g] - less, by = factor(g);
+                        const uint64_t c2 = pair(by, by), d2 = pair(term, term);
+                        uint64_t s2 = 0;
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) {
+                            float2 e = unpair(fma2(pair(__uint_as_float(v[x][16 * h + 2 * y]), __uint_as_float(v[x][16 * h + 2 * y + 1])), c2, d2));
+                            e.x = ex2(e.x);
+                            e.y = ex2(e.y);
+                            s2 = add2(s2, pair(e.x, e.y));
+                            w[8 * h + y] = half_pair(e.x, e.y);
+                        }
+                        const float2 q = unpair(s2);
+                        sum = fmaf(q.x + q.y, scale[16 + g], sum);
+                    }
+                    tmem_st16(tmem_s + x * 16, w);
+                    if (x & 1) {      // half of the weights: the products of their keys may begin
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(x == 1 ? bar_pa : bar_pb) : "memory");
+                    }
+                }
+            }
+            if (!ok) break;
+            ok = all_wait(bar_pv, np & 1u);
+            ++np;
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const bool begins = at.at >= mine.lo, whole = begins && at.at + at.slabs <= mine.hi;
+            float* partial = p.partials + (((uint64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * BT_ROWS + r) * (vdim + 2);
+            const float by = whole ? sum == 0.0f ? 0.0f : __fdiv_rn(back, sum) : back;
+            auto out_of = [&](uint32_t row) {
+                const uint32_t flat = at.tile * BT_ROWS + row;
+                return (uint64_t)(at.first_row + flat / group) * a.ld + (uint64_t)(at.head * group + flat % group) * vdim;
+            };
+            const bool wide = ((uintptr_t)a.out & 15u) == 0 && (a.ld & 7u) == 0;
+            const uint64_t out = r < rows ? out_of(r) : 0;
+            for (uint32_t x = 0; x < vdim; x += 16) {
+                uint32_t o[16];
+                tmem_ld16(tmem_o + x, o);
+                float f[16];
+#pragma unroll
+                for (int y = 0; y < 16; ++y) f[y] = __uint_as_float(o[y]) * by;
+                if (r >= rows) {
+                } else if (!whole) {
+#pragma unroll
+                    for (int y = 0; y < 16; y += 2) __stcg(reinterpret_cast<float2*>(partial + x + y), make_float2(f[y], f[y + 1]));
+                } else if (wide) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) w[y] = a.dtype == HOLO_DTYPE_F16 ? half_pair(f[2 * y], f[2 * y + 1]) : pack_bf16(f[2 * y], f[2 * y + 1]);
+                    uint4* to = reinterpret_cast<uint4*>((uint16_t*)a.out + out + x);
+                    to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                    to[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                } else {
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) seq_store(a.out, out + x + y, f[y], a.dtype);
+                }
+            }
+            __syncwarp();
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (!whole) {
+                if (r < rows) __stcg(reinterpret_cast<float2*>(partial + vdim), make_float2(top, sum));
+                // the plane's CTAs, and its counter: that of the CTA it begins in
+                const uint32_t from_cta = mine.first_cta(at), count = mine.cta_count(at);
+                arrive_at(bar_rows);
+                ok = all_wait(bar_rows, met++ & 1u);
+                if (!ok) break;
+                if (r == 0) {
+                    uint32_t n;
+                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(n) : "l"(p.arrivals + from_cta) : "memory");
+                    *s_last = n + 1 == count;
+                    if (n + 1 == count) p.arrivals[from_cta] = 0;
+                }
+                arrive_at(bar_rows);
+                ok = all_wait(bar_rows, met++ & 1u);
+                if (!ok) break;
+                if (*reinterpret_cast<volatile uint32_t*>(s_last)) {
+                    // a warp a row, two columns a lane and turn
+                    const uint32_t step = 2 * BT_ROWS * (vdim + 2), own = BT_ROWS * (vdim + 2);
+                    const float* first = p.partials + (uint64_t)from_cta * step;
+                    auto part = [&](uint32_t w, uint32_t row) { return first + (uint64_t)w * step + (w == 0 ? own : 0u) + row * (vdim + 2); };
+#pragma unroll 2
+                    for (uint32_t row = quarter; row < rows; row += 4) {
+                        float m = -INFINITY, l = 0.0f;
+                        for (uint32_t w = lane; w < count; w += 32) m = fmaxf(m, __ldcg(part(w, row) + vdim));
+                        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+                        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 4
+                        for (uint32_t w = 0; w < count; ++w) {
+                            const float* of = part(w, row);
+                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(of + vdim));
+                            const float f = ml.y == 0.0f ? 0.0f : ex2(ml.x - m);       // NaN is not 0
+                            l = fmaf(f, ml.y, l);
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const uint32_t col = 2 * lane + 64 * x;
+                                if (col >= vdim) continue;
+                                const float2 y = __ldcg(reinterpret_cast<const float2*>(of + col));
+                                acc[x] = make_float2(fmaf(f, y.x, acc[x].x), fmaf(f, y.y, acc[x].y));
+                            }
+                        }
+                        const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+                        const uint64_t to = out_of(row);
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t col = 2 * lane + 64 * x;
+                            if (col >= vdim) continue;
+                            const float lo = acc[x].x * inv, hi = acc[x].y * inv;
+                            if (wide) {
+                                *reinterpret_cast<uint32_t*>((uint16_t*)a.out + to + col) = a.dtype == HOLO_DTYPE_F16 ? half_pair(lo, hi) : pack_bf16(lo, hi);
+                            } else {
+                                seq_store(a.out, to + col, lo, a.dtype);
+                                seq_store(a.out, to + col + 1, hi, a.dtype);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        } while (more(at));
+    }
+    // everyone meets here, whatever happened above, so that TMEM is always released
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(256u) : "memory");
+    }
+}
+
+template <int UNITS>
+int32_t launch_block_tile(holo_b200_ctx* ctx, const BlockTileParams& p) {
+    const uint32_t smem = 1024 + 3 * p.k_chunks * TILE_CHUNK + 2 * p.v_chunks * TILE_CHUNK + 256 + 2 * BT_ROWS * 4 + 4 * 24 * 4;
+    static thread_local int configured_device = -1;
+    if (configured_device != ctx->device) {
+        HOLO_CUDA(cudaFuncSetAttribute(block_tile_kernel<UNITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, ctx->smem_optin));
+        configured_device = ctx->device;
+    }
+    HOLO_CUDA(holo_launch_kernel(ctx, block_tile_kernel<UNITS>, dim3((uint32_t)ctx->sm_count), dim3(BT_WARPS * 32), smem, 1, p));
+    ctx->launches++;
+    return HOLO_OK;
+}
+
+}  // namespace
+
+int32_t holo_try_block_tile(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool* taken) {
+    *taken = false;
+    const HoloBlockCache& c = a.c;
+    const uint32_t group = a.heads / c.kv_heads;
+    if (a.dtype == HOLO_DTYPE_F32 || c.block_rows % 16 != 0) return HOLO_OK;
+    if (c.dim % 16 != 0 || c.vdim % 16 != 0 || c.dim > 128 || c.vdim > 128 || (((uintptr_t)c.k_codes | (uintptr_t)c.v_codes) & 15u) != 0) return HOLO_OK;
+    // where a sequence has more rows of a head than the few-row kernel takes in three passes over the cache
+    if ((uint64_t)c.rows * group <= 24ull * c.sequences) return HOLO_OK;
+    // tiles of the whole list of 32 bits
+    const uint64_t tiles = ((uint64_t)c.rows * group / BT_ROWS + c.sequences) * c.kv_heads;
+    if ((uint64_t)c.rows * a.heads > 0x7fffffffull || tiles > 0x7fffffffull / (((uint64_t)c.table_ld * c.block_rows + BT_TILE - 1) / BT_TILE)) return HOLO_OK;
+    HOLO_TRY(holo_block_row_partials(ctx));
+    *taken = true;
+    BlockTileParams p = {};
+    p.a = a;
+    p.partials = ctx->block_row_partials;
+    p.arrivals = ctx->attn_arrivals;
+    p.group = group;
+    p.k_chunks = (c.dim + 63) / 64;
+    p.v_chunks = (c.vdim + 63) / 64;
+    p.br_shift = -1;
+    for (int s = 0; s <= 10; ++s)
+        if (c.block_rows == 1u << s) p.br_shift = s;
+    return c.dim <= 64 && c.vdim <= 64 ? launch_block_tile<4>(ctx, p) : launch_block_tile<8>(ctx, p);
+}

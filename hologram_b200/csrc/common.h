@@ -434,7 +434,9 @@ struct HoloBlockAttnArgs {
 int32_t holo_launch_block_cache_attention(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a);
 // block_attention.cu: dims in steps of 16; *taken false: the shape is not one it serves
 int32_t holo_try_block_attention(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool* taken);
-// block_rows.cu: many rows of a sequence
+// block_tile.cu, block_rows.cu: many rows of a sequence, in 16 bits and in any type
+int32_t holo_try_block_tile(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool* taken);
+int32_t holo_block_row_partials(holo_b200_ctx* ctx);
 int32_t holo_try_block_rows(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool* taken);
 // logit_rules.cu
 struct HoloLogitRulesArgs {

@@ -16,7 +16,7 @@
 //
 // A weight of zero times an infinite or NaN value is NaN, so a value that is not finite spoils its column in every row of the tile. A
 // row that ends with results that are not finite is computed again from memory by its own thread (redo_rows), only the keys it sees.
-#include "attention_tile.cuh"
+#include "attention_issue.cuh"
 #include "sequences.cuh"
 
 namespace {
@@ -40,27 +40,6 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 }
 template <bool F16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) { return F16 ? pack_half(lo, hi) : pack_bf16(lo, hi); }
-
-// The issuer runs with all its lanes and one of them is elected by a predicate, never by a branch: descriptors then stay in uniform registers,
-// where the instruction wants them. Behind a branch each product cost the thread 100 cycles, half as much again as the tensor core.
-__device__ __forceinline__ void elected_ss(uint32_t elected, uint32_t tmem_d, uint32_t a, uint32_t a_high, uint32_t b, uint32_t b_high, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n.reg .pred p, e;\n.reg .b64 x, y;\nmov.b64 x, {%1, %2};\nmov.b64 y, {%3, %4};\nsetp.ne.b32 e, %7, 0;\nsetp.ne.b32 p, %6, 0;\n"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, p;\n}\n"
-        ::"r"(tmem_d), "r"(a), "r"(a_high), "r"(b), "r"(b_high), "r"(idesc), "r"(accumulate), "r"(elected)
-        : "memory");
-}
-__device__ __forceinline__ void elected_ts(uint32_t elected, uint32_t tmem_d, uint32_t tmem_a, uint32_t b, uint32_t b_high, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n.reg .pred p, e;\n.reg .b64 y;\nmov.b64 y, {%2, %3};\nsetp.ne.b32 e, %6, 0;\nsetp.ne.b32 p, %5, 0;\n"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n}\n"
-        ::"r"(tmem_d), "r"(tmem_a), "r"(b), "r"(b_high), "r"(idesc), "r"(accumulate), "r"(elected)
-        : "memory");
-}
-__device__ __forceinline__ void elected_commit(uint32_t elected, uint32_t bar) {
-    asm volatile("{\n.reg .pred e;\nsetp.ne.b32 e, %1, 0;\n@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar), "r"(elected) : "memory");
-}
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // An item: the query tiles of a pair and a head. Tile q walks the key tiles [from[q], to[q]) of 128 keys each, counted from `anchor`;
 // left[q]: keys from there to its last one. Pairs come in the order of their work, the most first (many pairs: the last rows
@@ -144,18 +123,6 @@ __device__ __noinline__ void redo_rows(const PackedTileParams& p, uint32_t row, 
 #pragma unroll
     for (int c = 0; c < 64; ++c)
         if (2 * c < a.vdim) out[c] = sum == 0.0f ? 0u : pack16<F16>(__fdiv_rn(acc[2 * c], sum), __fdiv_rn(acc[2 * c + 1], sum));
-}
-
-// The wait of this kernel: the others may have to wait while a warp does rows again, so the limit is some seconds.
-__device__ __forceinline__ bool pt_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* status) {
-    for (uint32_t it = 0; it < (1u << 25); ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (*abort_flag) return false;
-        if (it > 64) __nanosleep(64);
-    }
-    *abort_flag = 1;
-    atomicOr(status, 4u);
-    return false;
 }
 
 constexpr float PT_WILD = 0x1p22f;     // from here on a fused exponent of the largest score is off by whole units
@@ -277,7 +244,7 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 const PackedItem it = item_of(i);
                 if (it.tiles == 0) continue;
                 const int g = (int)(it.head / (a.heads / a.kv_heads));
-                ok = nq == 0 || pt_wait(bar_q_empty, (nq - 1) & 1u, s_abort, a.status);
+                ok = nq == 0 || long_wait(bar_q_empty, (nq - 1) & 1u, s_abort, a.status);
                 if (!ok) break;
                 mbar_arrive_expect_tx(bar_q_full, p.nq * k_bytes);
                 for (uint32_t q = 0; q < p.nq; ++q)
@@ -285,13 +252,13 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                         tma_load_3d(s_q + q * k_bytes + c * TILE_CHUNK, &map_q, (int)(64 * c), (int)it.head, (int)(it.row0 + q * 128), bar_q_full);
                 ++nq;
                 for (uint32_t t = 0; t < it.tiles; ++t) {
-                    ok = nk < 2 || pt_wait(bar_k_empty + 8 * (nk & 1u), ((nk >> 1) - 1) & 1u, s_abort, a.status);
+                    ok = nk < 2 || long_wait(bar_k_empty + 8 * (nk & 1u), ((nk >> 1) - 1) & 1u, s_abort, a.status);
                     if (!ok) break;
                     mbar_arrive_expect_tx(bar_k_full + 8 * (nk & 1u), k_bytes);
                     for (uint32_t c = 0; c < p.k_chunks; ++c)
                         tma_load_3d(s_k + (nk & 1u) * k_bytes + c * TILE_CHUNK, &map_k, (int)(64 * c), g, (int)(it.anchor + t * 128), bar_k_full + 8 * (nk & 1u));
                     ++nk;
-                    ok = nv < 2 || pt_wait(bar_v_empty + 8 * (nv & 1u), ((nv >> 1) - 1) & 1u, s_abort, a.status);
+                    ok = nv < 2 || long_wait(bar_v_empty + 8 * (nv & 1u), ((nv >> 1) - 1) & 1u, s_abort, a.status);
                     if (!ok) break;
                     mbar_arrive_expect_tx(bar_v_full + 8 * (nv & 1u), v_bytes);
                     for (uint32_t c = 0; c < p.v_chunks; ++c)
@@ -323,7 +290,7 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             const uint32_t ksteps = KS ? KS : a.dim / 16;
             uint32_t nq = 0, nk = 0, nv = 0, np = 0;
             bool ok = true;
-            auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, pt_wait(bar, parity, s_abort, a.status)); };
+            auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, long_wait(bar, parity, s_abort, a.status)); };
             for (uint32_t i = 0; i < rounds && ok; ++i) {
                 const PackedItem it = item_of(i);
                 const uint32_t from = uniform(it.from[q]), to = uniform(it.to[q]), left = uniform(it.left[q]), tiles = uniform(it.tiles);
@@ -398,7 +365,7 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             const uint32_t all_from = __reduce_max_sync(0xffffffffu, mine ? begin : 0u), all_to = __reduce_min_sync(0xffffffffu, mine ? end : 0xffffffffu);
             float top = -INFINITY, sum = 0.0f;
             for (uint32_t t = from; t < to; ++t, ++ns) {
-                ok = pt_wait(bar_s + 8 * q, ns & 1u, s_abort, a.status) && !*s_abort;
+                ok = long_wait(bar_s + 8 * q, ns & 1u, s_abort, a.status) && !*s_abort;
                 ok = __all_sync(0xffffffffu, ok);   // the TMEM accesses below are whole-warp instructions
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -473,7 +440,7 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 const float2 s0 = unpair(add2(s2[0], s2[1]));
                 sum += s0.x + s0.y;
             }
-            ok = ok && pt_wait(bar_pv + 8 * q, ndone & 1u, s_abort, a.status) && !*s_abort;
+            ok = ok && long_wait(bar_pv + 8 * q, ndone & 1u, s_abort, a.status) && !*s_abort;
             ++ndone;
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;

@@ -584,7 +584,8 @@ typedef struct HoloPackedAttentionCall {
 } HoloPackedAttentionCall;
 
 /* The int8 block cache of the two calls below: codes i8 [blocks, kv_heads, block_rows, dim (k) or vdim (v)], scales f32 [blocks,
- * kv_heads] each for k and v; the value held is code * scale. table i32 [sequences, table_ld]: position p of sequence s is row
+ * kv_heads] each for k and v, finite and not negative; the value held is code * scale (value scales 2^-20 of the largest of their sequence and
+ * head and less may lose bits in attention). table i32 [sequences, table_ld]: position p of sequence s is row
  * p % block_rows of block table[s, p / block_rows]. lengths i32 [sequences]: the positions of each sequence, those of the call's rows
  * included. The call's rows are packed: sequence s has rows [starts[s], starts[s + 1]), which are its last positions (starts absent:
  * row s is the one row of sequence s, and `rows` is `sequences`). Entries of the table behind a sequence's positions are not read.

@@ -358,6 +358,13 @@ CACHES = [
     ([1, 4], [300, 3], 48, 20, 1, 80, 512),
     ([1], [5000], 16, 16, 2, 128, 128),
     ([64], [700], 16, 48, 2, 64, 128),
+    # portions: many rows of a sequence
+    ([200, 5, 70], [1000, 0, 333], 64, 8, 2, 96, 48),
+    ([130], [0], 16, 4, 4, 64, 64),
+    ([33, 257, 0, 80], [129, 64, 7, 1500], 48, 6, 2, 80, 112),
+    ([90, 31], [37, 600], 24, 4, 1, 128, 128),      # blocks that are no multiple of 16 rows
+    ([1, 300, 1, 1], [2000, 5, 0, 127], 32, 8, 1, 128, 64),
+    ([128], [2944], 128, 4, 1, 16, 16),
 ]
 
 
