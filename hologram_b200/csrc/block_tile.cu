@@ -22,7 +22,7 @@ constexpr int BT_LIFT = 7;
 
 struct BlockTileParams {
     HoloBlockAttnArgs a;
-    float* partials;          // [CTAs][2][128 rows][vdim + 2]
+    float* partials;          // [CTAs][2][vdim + 2][128 rows]: a warp's rows side by side
     uint32_t* arrivals;       // a counter per CTA, zero between launches
     uint32_t group, k_chunks, v_chunks;      // chunks of 64 columns
     int32_t br_shift;
@@ -30,8 +30,6 @@ struct BlockTileParams {
 
 constexpr uint32_t PICK01 = 0x4140, PICK23 = 0x4342;
 
-// UNITS: 16-byte units of codes of a row, at most; a worker thread has one key and all its units
-template <int UNITS>
 __global__ void __launch_bounds__(BT_WARPS * 32, 1)
 block_tile_kernel(const __grid_constant__ BlockTileParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -99,12 +97,13 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
 
     if (warp >= 8) {
         // ---------------- workers: codes and queries into operands ----------------
-        const uint32_t me = tid - 8 * 32;
+        // eight lanes take the 16-byte units of a row of codes, a warp four rows at a time: unit `unit` of keys 16 j + sub
+        const uint32_t me = tid - 8 * 32, unit = lane & 7u, sub = (warp - 8) * 4 + (lane >> 3);
         uint32_t nt = 0, np = 0;
         bool ok = true;
         auto block_of = [&](uint32_t pos) { return p.br_shift >= 0 ? pos >> p.br_shift : pos / br; };
         // 16 codes as 32 bytes of a 128-byte row: the row's 16-byte units stand at their number xor key % 8
-        auto turn = [&](uint8_t* tile, uint32_t unit, const uint4& v) {
+        auto turn = [&](uint8_t* tile, uint32_t key, const uint4& v) {
             const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
             uint32_t h[8];
 #pragma unroll
@@ -112,9 +111,9 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                 h[2 * e] = codes_to_half<PICK01>(w[e]);
                 h[2 * e + 1] = codes_to_half<PICK23>(w[e]);
             }
-            uint4* to = reinterpret_cast<uint4*>(tile + (unit >> 2) * TILE_CHUNK + me * 128);
-            to[(2 * (unit & 3u)) ^ (me & 7u)] = make_uint4(h[0], h[1], h[2], h[3]);
-            to[(2 * (unit & 3u) + 1) ^ (me & 7u)] = make_uint4(h[4], h[5], h[6], h[7]);
+            uint4* to = reinterpret_cast<uint4*>(tile + (unit >> 2) * TILE_CHUNK + key * 128);
+            to[(2 * (unit & 3u)) ^ (key & 7u)] = make_uint4(h[0], h[1], h[2], h[3]);
+            to[(2 * (unit & 3u) + 1) ^ (key & 7u)] = make_uint4(h[4], h[5], h[6], h[7]);
         };
         auto arrive = [&](uint32_t bar) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -125,37 +124,55 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
             uint32_t s0, s1;
             mine.ends_of(at, &s0, &s1);
             const uint32_t sees = keys_of(at), rows = min((uint32_t)BT_ROWS, at.n * group - at.tile * BT_ROWS);
-            // the block that holds this thread's key of a tile, or -1
+            // Sixteen keys in a row lie in one block: lane j < 8 has the number of the block of keys 16 j of a tile, as the table has it
             auto find = [&](uint32_t tile) {
-                const uint32_t pos = tile * BT_TILE + me;
-                if (tile >= s1 || pos >= sees) return -1;
-                const int id = c.table[(uint64_t)at.seq * c.table_ld + block_of(pos)];
-                if ((uint32_t)id < c.blocks) return id;
-                atomicOr(c.status, HOLO_STATUS_TABLE);
-                return -1;
+                const uint32_t pos = tile * BT_TILE + 16 * lane;
+                return lane < 8 && tile < s1 && pos < sees ? c.table[(uint64_t)at.seq * c.table_ld + block_of(pos)] : -1;
             };
-            int id = find(s0), next_id = find(s0 + 1);
-            uint4 kreg[UNITS], vreg[UNITS];
+            // where those keys' rows begin in the cache, none: 0xffffffff
+            auto rows_of = [&](uint32_t tile, int id) {
+                const uint32_t pos = tile * BT_TILE + 16 * lane;
+                if (lane >= 8 || tile >= s1 || pos >= sees) return 0xffffffffu;
+                if ((uint32_t)id >= c.blocks) {
+                    atomicOr(c.status, HOLO_STATUS_TABLE);
+                    return 0xffffffffu;
+                }
+                return ((uint32_t)id * c.kv_heads + at.head) * br + (pos - block_of(pos) * br);
+            };
+            uint4 kreg[8], vreg[8];
             float ks = 0.0f, vs = 0.0f;
-            auto row_of = [&](uint32_t tile, int b) {
-                const uint32_t pos = tile * BT_TILE + me;
-                return ((uint64_t)(uint32_t)b * c.kv_heads + at.head) * br + (pos - block_of(pos) * br);
-            };
-            auto load_k = [&](uint32_t tile, int b) {
-                const uint4* from = reinterpret_cast<const uint4*>(c.k_codes + (b < 0 ? 0 : row_of(tile, b) * dim));
+            auto load_codes = [&](uint4 (&to)[8], const int8_t* codes, uint32_t d, uint32_t from) {
 #pragma unroll
-                for (int u = 0; u < UNITS; ++u) kreg[u] = b >= 0 && 16 * u < dim ? from[u] : make_uint4(0, 0, 0, 0);
-                const uint64_t plane = (uint64_t)(uint32_t)max(b, 0) * c.kv_heads + at.head;
-                ks = b < 0 ? 0.0f : c.k_scales[plane];
-                vs = b < 0 ? 0.0f : c.v_scales[plane];
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t row = __shfl_sync(0xffffffffu, from, j);
+                    to[j] = row != 0xffffffffu && 16 * unit < d ? *reinterpret_cast<const uint4*>(codes + (uint64_t)(row + sub) * d + 16 * unit) : make_uint4(0, 0, 0, 0);
+                }
             };
-            auto load_v = [&](uint32_t tile, int b) {
-                const uint4* from = reinterpret_cast<const uint4*>(c.v_codes + (b < 0 ? 0 : row_of(tile, b) * vdim));
+            auto load_scales = [&](uint32_t from) {
+                const bool there = from != 0xffffffffu;
+                const uint32_t plane = there ? from / br : 0u;
+                ks = there ? c.k_scales[plane] : 0.0f;
+                vs = there ? c.v_scales[plane] : 0.0f;
+            };
+            uint32_t from = rows_of(s0, find(s0));
+            int ahead = find(s0 + 1);
+            load_codes(kreg, c.k_codes, dim, from);
+            load_codes(vreg, c.v_codes, vdim, from);
+            load_scales(from);
+            // this warp's query rows are on their way while the rest of the plane's beginning is done
+            const uint32_t row0 = (warp - 8) * 32;
+            const bool wide_q = ((uintptr_t)a.q & 7u) == 0 && (a.q_ld & 3u) == 0;
+            uint2 query[16];
+            auto load_query = [&](uint32_t r) {
+                const uint32_t flat = at.tile * BT_ROWS + r, i = flat / group;
+                const uint64_t q = (uint64_t)(at.first_row + i) * a.q_ld + (uint64_t)(at.head * group + flat - i * group) * dim + 4 * lane;
+                if (r >= rows || 4 * lane >= dim) return make_uint2(0, 0);
+                const uint16_t* from_q = (const uint16_t*)a.q + q;
+                if (wide_q) return *reinterpret_cast<const uint2*>(from_q);
+                return make_uint2(from_q[0] | (uint32_t)from_q[1] << 16, from_q[2] | (uint32_t)from_q[3] << 16);
+            };
 #pragma unroll
-                for (int u = 0; u < UNITS; ++u) vreg[u] = b >= 0 && 16 * u < vdim ? from[u] : make_uint4(0, 0, 0, 0);
-            };
-            load_k(s0, id);
-            load_v(s0, id);
+            for (int r = 0; r < 16; ++r) query[r] = load_query(row0 + r);
             // the largest value scale of the CTA's part of the plane
             float largest = 0.0f;
             for (uint32_t b = block_of(s0 * BT_TILE) + me, last = block_of(min(s1 * BT_TILE, sees) - 1); b <= last; b += BT_WORKERS) {
@@ -173,47 +190,48 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
             const uint32_t top_bits = max(max(most_of[0], most_of[1]), max(most_of[2], most_of[3]));
             const int lift = max((int)(top_bits >> 23) - 126, -100);       // 2^lift is above it
             if (me == 0) s_lift[np & 1u] = lift;
-            // query rows, a warp a row at a time: all lanes a row's columns
-            const uint32_t halves = dim / 2;
-#pragma unroll 4
-            for (uint32_t r = (warp - 8) * 32; r < (warp - 8) * 32 + 32; ++r) {
-                const uint32_t flat = at.tile * BT_ROWS + r, i = flat / group, head = at.head * group + flat % group;
-                float2 x[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                float most = 0.0f;
-                bool finite = true;
+            // query rows, a warp a row at a time, four columns a lane: 16 lanes are a chunk of 64 columns, two lanes a unit
+#pragma unroll 1
+            for (uint32_t h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t d = lane + 32 * e;
-                    if (r < rows && d < halves) {
-                        const uint64_t q = (uint64_t)(at.first_row + i) * a.q_ld + (uint64_t)head * dim + 2 * d;
-                        x[e] = make_float2(seq_load(a.q, q, a.dtype), seq_load(a.q, q + 1, a.dtype));
+                for (int n = 0; n < 16; ++n) {
+                    const uint32_t r = row0 + 16 * h + n;
+                    const uint2 v = query[n];
+                    float x[4];
+                    if (a.dtype == HOLO_DTYPE_BF16) {
+                        x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
+                        x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+                    } else {
+                        const float2 lo = half_values(v.x), hi = half_values(v.y);
+                        x[0] = lo.x; x[1] = lo.y; x[2] = hi.x; x[3] = hi.y;
                     }
-                    most = fmaxf(most, fmaxf(fabsf(x[e].x), fabsf(x[e].y)));
-                    finite = finite && fabsf(x[e].x) < INFINITY && fabsf(x[e].y) < INFINITY;
-                }
-                const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-                finite = __all_sync(0xffffffffu, finite);
-                // 2^e <= most < 2^(e + 1); two factors, since 2^(14 - e) alone may overflow
-                const int up = finite && m ? 14 - (m >> 23 ? (int)(m >> 23) - 127 : -118 - __clz((int)m)) : 0;
-                const float f0 = power_of_two(up / 2), f1 = power_of_two(up - up / 2);
+                    // magnitudes order as their bits do, infinities and NaN above all
+                    uint32_t most = 0;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t d = lane + 32 * e;       // pair of columns: 32 pairs are a chunk of 64 columns, 4 pairs a unit
-                    if (d < halves)
-                        *reinterpret_cast<uint32_t*>(sm + e * TILE_CHUNK + r * 128 + (((lane >> 2) ^ (r & 7u)) << 4) + 4 * (lane & 3u)) =
-                            finite ? half_pair(x[e].x * f0 * f1, x[e].y * f0 * f1) : 0u;
+                    for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+                    most = __reduce_max_sync(0xffffffffu, most);
+                    const bool finite = most < 0x7f800000u;
+                    // 2^e <= most < 2^(e + 1); two factors, since 2^(14 - e) alone may overflow
+                    const int up = finite && most ? 14 - (most >> 23 ? (int)(most >> 23) - 127 : -118 - __clz((int)most)) : 0;
+                    const float f0 = power_of_two(up / 2), f1 = power_of_two(up - up / 2);
+                    if (4 * lane < dim)
+                        *reinterpret_cast<uint2*>(sm + (lane >> 4) * TILE_CHUNK + r * 128 + (((lane >> 1 & 7u) ^ (r & 7u)) << 4) + 8 * (lane & 1u)) =
+                            finite ? make_uint2(half_pair(x[0] * f0 * f1, x[1] * f0 * f1), half_pair(x[2] * f0 * f1, x[3] * f0 * f1)) : make_uint2(0, 0);
+                    if (lane == 0) s_row[(np & 1u) * BT_ROWS + r] = finite ? a.scale * LOG2E * power_of_two(-(up / 2)) * power_of_two(-(up - up / 2)) : NAN;
                 }
-                if (lane == 0) s_row[(np & 1u) * BT_ROWS + r] = finite ? a.scale * LOG2E * power_of_two(-(up / 2)) * power_of_two(-(up - up / 2)) : NAN;
+                if (h == 0)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) query[r] = load_query(row0 + 16 + r);
             }
             arrive(bar_q_full);
             ++np;
 #pragma unroll 1
             for (uint32_t t = s0; t < s1 && ok; ++t, ++nt) {
                 const uint32_t stage = nt & 1u;
-                // scales of 16 keys in a row, from the thread that has the first of them. A value scale 2^-60 of the largest and less is as good
+                // scales of 16 keys in a row, from the lane that has their block. A value scale 2^-60 of the largest and less is as good
                 // as none; its keys' weights still count in the rows' sums
-                if ((me & 15u) == 0) {
-                    float* to = s_scale + (nt & 3u) * 24 + (me >> 4);
+                if (me < 8) {
+                    float* to = s_scale + (nt & 3u) * 24 + me;
                     const float x = fmaxf(vs, power_of_two(max(lift - 60, -126)));
                     to[0] = ks;
                     to[8] = __log2f(x) + (float)(BT_LIFT - lift);
@@ -221,20 +239,21 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                 }
                 ok = nt < 2 || all_wait(bar_k_empty + 8 * stage, ((nt >> 1) - 1) & 1u);
                 if (!ok) break;
+                if (16 * unit < dim)
 #pragma unroll
-                for (int u = 0; u < UNITS; ++u)
-                    if (16 * u < dim) turn(sm + o_k + stage * k_bytes, u, kreg[u]);
+                    for (int j = 0; j < 8; ++j) turn(sm + o_k + stage * k_bytes, 16 * j + sub, kreg[j]);
                 arrive(bar_k_full + 8 * stage);
-                const int after = find(t + 2);
-                load_k(t + 1, next_id);
+                from = rows_of(t + 1, ahead);
+                ahead = find(t + 2);
+                load_codes(kreg, c.k_codes, dim, from);
+                load_scales(from);
                 ok = nt < 2 || all_wait(bar_v_empty + 8 * stage, ((nt >> 1) - 1) & 1u);
                 if (!ok) break;
+                if (16 * unit < vdim)
 #pragma unroll
-                for (int u = 0; u < UNITS; ++u)
-                    if (16 * u < vdim) turn(sm + o_v + stage * v_bytes, u, vreg[u]);
+                    for (int j = 0; j < 8; ++j) turn(sm + o_v + stage * v_bytes, 16 * j + sub, vreg[j]);
                 arrive(bar_v_full + 8 * stage);
-                load_v(t + 1, next_id);
-                next_id = after;
+                load_codes(vreg, c.v_codes, vdim, from);
             }
         } while (ok && more(at));
     } else if (warp == 1) {
@@ -405,7 +424,7 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const bool begins = at.at >= mine.lo, whole = begins && at.at + at.slabs <= mine.hi;
-            float* partial = p.partials + (((uint64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * BT_ROWS + r) * (vdim + 2);
+            float* partial = p.partials + ((uint64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * BT_ROWS * (vdim + 2) + r;
             const float by = whole ? sum == 0.0f ? 0.0f : __fdiv_rn(back, sum) : back;
             auto out_of = [&](uint32_t row) {
                 const uint32_t flat = at.tile * BT_ROWS + row;
@@ -413,6 +432,19 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
             };
             const bool wide = ((uintptr_t)a.out & 15u) == 0 && (a.ld & 7u) == 0;
             const uint64_t out = r < rows ? out_of(r) : 0;
+            auto store16 = [&](uint64_t index, const float (&f)[16]) {
+                if (wide) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) w[y] = a.dtype == HOLO_DTYPE_F16 ? half_pair(f[2 * y], f[2 * y + 1]) : pack_bf16(f[2 * y], f[2 * y + 1]);
+                    uint4* to = reinterpret_cast<uint4*>((uint16_t*)a.out + index);
+                    to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                    to[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                } else {
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) seq_store(a.out, index + y, f[y], a.dtype);
+                }
+            };
             for (uint32_t x = 0; x < vdim; x += 16) {
                 uint32_t o[16];
                 tmem_ld16(tmem_o + x, o);
@@ -422,23 +454,18 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                 if (r >= rows) {
                 } else if (!whole) {
 #pragma unroll
-                    for (int y = 0; y < 16; y += 2) __stcg(reinterpret_cast<float2*>(partial + x + y), make_float2(f[y], f[y + 1]));
-                } else if (wide) {
-                    uint32_t w[8];
-#pragma unroll
-                    for (int y = 0; y < 8; ++y) w[y] = a.dtype == HOLO_DTYPE_F16 ? half_pair(f[2 * y], f[2 * y + 1]) : pack_bf16(f[2 * y], f[2 * y + 1]);
-                    uint4* to = reinterpret_cast<uint4*>((uint16_t*)a.out + out + x);
-                    to[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                    to[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                    for (int y = 0; y < 16; ++y) __stcg(partial + (x + y) * BT_ROWS, f[y]);
                 } else {
-#pragma unroll
-                    for (int y = 0; y < 16; ++y) seq_store(a.out, out + x + y, f[y], a.dtype);
+                    store16(out + x, f);
                 }
             }
             __syncwarp();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (!whole) {
-                if (r < rows) __stcg(reinterpret_cast<float2*>(partial + vdim), make_float2(top, sum));
+                if (r < rows) {
+                    __stcg(partial + vdim * BT_ROWS, top);
+                    __stcg(partial + (vdim + 1) * BT_ROWS, sum);
+                }
                 // the plane's CTAs, and its counter: that of the CTA it begins in
                 const uint32_t from_cta = mine.first_cta(at), count = mine.cta_count(at);
                 arrive_at(bar_rows);
@@ -454,43 +481,32 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                 ok = all_wait(bar_rows, met++ & 1u);
                 if (!ok) break;
                 if (*reinterpret_cast<volatile uint32_t*>(s_last)) {
-                    // a warp a row, two columns a lane and turn
+                    // a thread its row
                     const uint32_t step = 2 * BT_ROWS * (vdim + 2), own = BT_ROWS * (vdim + 2);
-                    const float* first = p.partials + (uint64_t)from_cta * step;
-                    auto part = [&](uint32_t w, uint32_t row) { return first + (uint64_t)w * step + (w == 0 ? own : 0u) + row * (vdim + 2); };
-#pragma unroll 2
-                    for (uint32_t row = quarter; row < rows; row += 4) {
+                    const float* first = p.partials + (uint64_t)from_cta * step + r;
+                    auto part = [&](uint32_t w) { return first + (uint64_t)w * step + (w == 0 ? own : 0u); };
+                    if (r < rows) {
                         float m = -INFINITY, l = 0.0f;
-                        for (uint32_t w = lane; w < count; w += 32) m = fmaxf(m, __ldcg(part(w, row) + vdim));
-                        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-                        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 4
+                        for (uint32_t w = 0; w < count; ++w) m = fmaxf(m, __ldcg(part(w) + vdim * BT_ROWS));
+                        auto weight = [&](uint32_t w, float sum_w) { return sum_w == 0.0f ? 0.0f : ex2(__ldcg(part(w) + vdim * BT_ROWS) - m); };      // NaN is not 0
 #pragma unroll 4
                         for (uint32_t w = 0; w < count; ++w) {
-                            const float* of = part(w, row);
-                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(of + vdim));
-                            const float f = ml.y == 0.0f ? 0.0f : ex2(ml.x - m);       // NaN is not 0
-                            l = fmaf(f, ml.y, l);
-#pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                const uint32_t col = 2 * lane + 64 * x;
-                                if (col >= vdim) continue;
-                                const float2 y = __ldcg(reinterpret_cast<const float2*>(of + col));
-                                acc[x] = make_float2(fmaf(f, y.x, acc[x].x), fmaf(f, y.y, acc[x].y));
-                            }
+                            const float lw = __ldcg(part(w) + (vdim + 1) * BT_ROWS);
+                            l = fmaf(weight(w, lw), lw, l);
                         }
                         const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-                        const uint64_t to = out_of(row);
+                        for (uint32_t x = 0; x < vdim; x += 16) {
+                            float acc[16];
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t col = 2 * lane + 64 * x;
-                            if (col >= vdim) continue;
-                            const float lo = acc[x].x * inv, hi = acc[x].y * inv;
-                            if (wide) {
-                                *reinterpret_cast<uint32_t*>((uint16_t*)a.out + to + col) = a.dtype == HOLO_DTYPE_F16 ? half_pair(lo, hi) : pack_bf16(lo, hi);
-                            } else {
-                                seq_store(a.out, to + col, lo, a.dtype);
-                                seq_store(a.out, to + col + 1, hi, a.dtype);
+                            for (int y = 0; y < 16; ++y) acc[y] = 0.0f;
+#pragma unroll 2
+                            for (uint32_t w = 0; w < count; ++w) {
+                                const float f = weight(w, __ldcg(part(w) + (vdim + 1) * BT_ROWS)) * inv;
+#pragma unroll
+                                for (int y = 0; y < 16; ++y) acc[y] = fmaf(f, __ldcg(part(w) + (x + y) * BT_ROWS), acc[y]);
                             }
+                            store16(out + x, acc);
                         }
                     }
                     __syncwarp();
@@ -508,15 +524,14 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
     }
 }
 
-template <int UNITS>
 int32_t launch_block_tile(holo_b200_ctx* ctx, const BlockTileParams& p) {
     const uint32_t smem = 1024 + 3 * p.k_chunks * TILE_CHUNK + 2 * p.v_chunks * TILE_CHUNK + 256 + 2 * BT_ROWS * 4 + 4 * 24 * 4;
     static thread_local int configured_device = -1;
     if (configured_device != ctx->device) {
-        HOLO_CUDA(cudaFuncSetAttribute(block_tile_kernel<UNITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, ctx->smem_optin));
+        HOLO_CUDA(cudaFuncSetAttribute(block_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ctx->smem_optin));
         configured_device = ctx->device;
     }
-    HOLO_CUDA(holo_launch_kernel(ctx, block_tile_kernel<UNITS>, dim3((uint32_t)ctx->sm_count), dim3(BT_WARPS * 32), smem, 1, p));
+    HOLO_CUDA(holo_launch_kernel(ctx, block_tile_kernel, dim3((uint32_t)ctx->sm_count), dim3(BT_WARPS * 32), smem, 1, p));
     ctx->launches++;
     return HOLO_OK;
 }
@@ -534,6 +549,7 @@ int32_t holo_try_block_tile(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool
     // tiles of the whole list of 32 bits
     const uint64_t tiles = ((uint64_t)c.rows * group / BT_ROWS + c.sequences) * c.kv_heads;
     if ((uint64_t)c.rows * a.heads > 0x7fffffffull || tiles > 0x7fffffffull / (((uint64_t)c.table_ld * c.block_rows + BT_TILE - 1) / BT_TILE)) return HOLO_OK;
+    if ((uint64_t)c.blocks * c.kv_heads * c.block_rows >= 0xffffffffull) return HOLO_OK;      // row numbers of 32 bits
     HOLO_TRY(holo_block_row_partials(ctx));
     *taken = true;
     BlockTileParams p = {};
@@ -546,5 +562,5 @@ int32_t holo_try_block_tile(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool
     p.br_shift = -1;
     for (int s = 0; s <= 10; ++s)
         if (c.block_rows == 1u << s) p.br_shift = s;
-    return c.dim <= 64 && c.vdim <= 64 ? launch_block_tile<4>(ctx, p) : launch_block_tile<8>(ctx, p);
+    return launch_block_tile(ctx, p);
 }
