@@ -692,3 +692,376 @@ def test_no_host_workspace_form(backend):
                  kc.KernelCall.BlockCacheAttention(kc.BlockCacheAttentionCall()), kc.KernelCall.LogitRules(kc.LogitRulesCall())):
         with pytest.raises(hb.BackendError, match="no host-workspace form"):
             backend.dispatch(call, host)
+
+
+# ---- the calls together, and what a caller may do around them ----------------------------------------------------------
+
+
+class Step:
+    """A step of several sequences: the rows' attention, their keys and values into the cache, and rules on logits, which here are the
+    attention's output of a row read as a vocabulary. `prompts` (packed attention) before the cache has anything, then single tokens."""
+
+    def __init__(self, rng, dtype, new, before, heads=8, kv=2, dim=64, block=16):
+        self.dtype, self.heads, self.kv, self.dim, self.new = dtype, heads, kv, dim, new
+        self.starts, rows, self.vocab = starts_of(new), int(sum(new)), heads * dim
+        self.before, self.after = before, [a + b for a, b in zip(new, before)]
+        self.qkv = strided(rng, rows, (heads + 2 * kv) * dim, (heads + 2 * kv) * dim, dtype)       # one product's columns
+        self.q, self.k, self.v = self.qkv[:, :heads * dim], self.qkv[:, heads * dim:(heads + kv) * dim], self.qkv[:, (heads + kv) * dim:]
+        self.out = torch.zeros(rows, self.vocab, dtype=TORCH[dtype], device="cuda")
+        self.history = rng.integers(0, self.vocab, (rows, 12)).astype(np.int32)
+        self.params = np.tile(np.array([[1.25, 0.5, 0.25, 0.5]], dtype=np.float32), (rows, 1))
+        self.masks = rng.integers(0, 2 ** 32, (rows, self.vocab // 32), dtype=np.uint64).astype(np.uint32)
+        self.logits = torch.zeros(rows, self.vocab, dtype=TORCH[dtype], device="cuda")
+        self.rule_args = [torch.from_numpy(self.history).cuda(), i32([[4, 12]] * rows), torch.from_numpy(self.params).cuda()]
+        self.dev_masks = torch.from_numpy(self.masks.view(np.int32)).cuda()
+
+    def calls(self, s, cache, prompt):
+        """The step's calls over the slots `s`, the cache's lengths being those after the step."""
+        rows, bare = self.q.shape[0], kc.NONE
+        starts = s(i32(list(map(int, self.starts)))) if prompt else None
+        q, k, v, out = s(self.q), s(self.k), s(self.v), s(self.out)
+        refs = cache.refs(s, None)
+        if prompt:
+            refs[0] = starts
+        sizes = (rows, len(self.new), self.kv, self.dim, self.dim, self.k.stride(0), self.v.stride(0), cache.block, cache.blocks, cache.width, TAG[self.dtype])
+        calls = [kc.KernelCall.BlockCacheWrite(kc.BlockCacheWriteCall(k, v, *refs, *sizes))]
+        if prompt:
+            calls.append(kc.KernelCall.PackedAttention(kc.PackedAttentionCall(q, k, v, starts, out, rows, len(self.new), self.heads, self.kv, self.dim, self.dim, self.q.stride(0),
+                                                                              self.k.stride(0), self.v.stride(0), self.vocab, 0, 1, TAG[self.dtype])))
+        else:
+            calls.append(kc.KernelCall.BlockCacheAttention(kc.BlockCacheAttentionCall(q, *refs, out, rows, len(self.new), self.heads, self.kv, self.dim, self.dim, self.q.stride(0),
+                                                                                      self.vocab, cache.block, cache.blocks, cache.width, 0, TAG[self.dtype])))
+        history, spans, params = (s(t) for t in self.rule_args)
+        calls.append(kc.KernelCall.LogitRules(kc.LogitRulesCall(out, history, spans, params, bare, bare, bare, s(self.dev_masks), bare, s(self.logits), rows, self.vocab, self.vocab,
+                                                                self.vocab, 12, 0, rows, self.vocab // 32, TAG[self.dtype])))
+        return calls
+
+    def check(self, cache, prompt):
+        """After the calls: the cache code for code, every row's logits within their bounds."""
+        rows, d = self.q.shape[0], self.dim
+        kf, vf = f64(self.k).reshape(rows, self.kv, d), f64(self.v).reshape(rows, self.kv, d)
+        write_plane(kf, cache.host["k_codes"], cache.host["k_scales"], self.starts, self.after, cache.table, cache.block)
+        write_plane(vf, cache.host["v_codes"], cache.host["v_scales"], self.starts, self.after, cache.table, cache.block)
+        same_cache(cache)
+        qf, got = f64(self.q).reshape(rows, self.heads, d), f64(self.logits)
+        for s, n in enumerate(self.after):
+            a, m = int(self.starts[s]), self.new[s]
+            k, v = (kf[a:a + m], vf[a:a + m]) if prompt else (cache.held("k", s, n), cache.held("v", s, n))
+            parts = [attend(qf[a:a + m, h], k[:, h // (self.heads // self.kv)], v[:, h // (self.heads // self.kv)], n - m + 1 + np.arange(m), d ** -0.5, self.dtype,
+                            (WEIGHT_HALF if prompt else CACHE_WEIGHT_HALF)[self.dtype]) for h in range(self.heads)]
+            for i in range(m):
+                z, z_off = (np.concatenate([p[part][i] for p in parts]) for part in (0, 1))
+                allowed = (self.masks[a + i][np.arange(self.vocab) >> 5] >> (np.arange(self.vocab) & 31).astype(np.uint32) & 1).astype(bool)
+                want, off = rules(z, self.history[a + i], (4, 12), self.params[a + i], [], allowed)
+                fine = np.isfinite(want)
+                assert np.array_equal(fine, np.isfinite(got[a + i]))
+                # an error of the attention's grows by the repetition's 1.25 and the temperature's 1 / 0.5 at most
+                check(got[a + i][fine], want[fine], (2.5 * z_off + 1.01 * off + HALF_STEP[self.dtype] * (np.abs(want) + 2.5 * z_off))[fine] + (2.0 ** -25 if self.dtype == "f16" else 0.0), f"row {a + i}")
+
+
+def serve(rng, dtype, dispatch, backend):
+    """Prompts of four sequences, then three single tokens of each: everything of a step is enqueued before anything is read."""
+    lens, block = [37, 1, 130, 16], 16
+    cache = Cache(rng, [n + 3 for n in lens], block, 2, 64, 64)
+    results = []
+    for turn in range(4):
+        new = lens if turn == 0 else [1] * 4
+        step = Step(rng, dtype, new, [0] * 4 if turn == 0 else [n + turn - 1 for n in lens], block=block)
+        cache.lens = step.after
+        s = Slots(backend, 24)
+        dispatch(step.calls(s, cache, turn == 0), s)
+        backend.synchronize()
+        step.check(cache, turn == 0)
+        results.append(step.logits.clone())
+    return results
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_a_served_batch_of_prompts_and_tokens(backend, dtype):
+    def dispatch(calls, s):
+        for c in calls:
+            backend.dispatch(c, s.ws)
+
+    serve(np.random.default_rng(21), dtype, dispatch, backend)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_a_served_batch_recorded_and_replayed(dtype):
+    """The same steps as graphs on another stream, each replayed twice: the calls write the same values again."""
+    be, stream = hb.B200Backend(0), torch.cuda.Stream()
+    be.set_stream(stream.cuda_stream)
+    kept = []
+
+    def direct(calls, s):
+        for c in calls:
+            be.dispatch(c, s.ws)
+
+    def recorded(calls, s):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+            for c in calls:
+                be.dispatch(c, s.ws)
+        with torch.cuda.stream(stream):
+            graph.replay()
+            graph.replay()
+        stream.synchronize()
+        kept.append((graph, s))
+
+    first = serve(np.random.default_rng(22), dtype, direct, be)
+    second = serve(np.random.default_rng(22), dtype, recorded, be)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    for graph, s in kept:
+        s.ws.close()
+    del graph
+    kept.clear()
+    be.close()
+
+
+def test_the_first_call_that_needs_a_buffer_is_not_recorded():
+    be, stream, rng = hb.B200Backend(0), torch.cuda.Stream(), np.random.default_rng(1)
+    be.set_stream(stream.cuda_stream)
+    for new in ([1, 1], [100, 40]):
+        cache = Cache(rng, [200, 100], 16, 2, 64, 64)
+        q, out = strided(rng, sum(new), 256, 256, "bf16"), torch.zeros(sum(new), 256, dtype=torch.bfloat16, device="cuda")
+        s = Slots(be, 12)
+        call = kc.KernelCall.BlockCacheAttention(kc.BlockCacheAttentionCall(s(q), *cache.refs(s, starts_of(new)), s(out), sum(new), 2, 4, 2, 64, 64, 256, 256, 16, cache.blocks, cache.width, 0,
+                                                                            kc.DTYPE_BF16))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+            with pytest.raises(hb.BackendError, match="first call") as e:
+                be.dispatch(call, s.ws)
+        assert e.value.variant == "Dispatch"
+        del e           # its traceback holds the workspace, which must not go in the middle of the next recording
+        be.dispatch(call, s.ws)
+        be.synchronize()
+        del graph
+        graph = torch.cuda.CUDAGraph()
+        want = out.clone()
+        with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+            be.dispatch(call, s.ws)
+        out.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        del graph
+    be.close()
+
+
+def archive_of(calls_of, tensors, outputs):
+    """A `.holo` image of `calls_of(slot references)` whose slots are input ports of the tensors' sizes, those of `outputs` output ports."""
+    from hologram_b200 import holo
+    w = holo.HoloWriter()
+    names = list(tensors)
+    refs = {n: kc.rb(i) for i, n in enumerate(names)}
+    w.calls.extend(calls_of(refs))
+    kinds = {torch.bfloat16: kc.DTYPE_BF16, torch.float16: kc.DTYPE_F16, torch.float32: kc.DTYPE_F32, torch.int32: kc.DTYPE_I32, torch.int8: kc.DTYPE_I8}
+    for i, n in enumerate(names):
+        t = tensors[n]
+        (w.outputs if n in outputs else w.inputs).append(holo.Port(n, i, t.numel(), kinds[t.dtype], list(t.shape)))
+    w.exec_plan = [[i] for i in range(len(w.calls))]
+    w.slot_bytes = [t.numel() * t.element_size() for t in tensors.values()]
+    return w.finish()
+
+
+def test_the_calls_through_an_archive_session(backend):
+    """One archive of write, attention and rules; walked, then recorded and replayed: the dispatched calls' bits. Addressed sessions refuse them."""
+    rng = np.random.default_rng(23)
+    rows, lens = 3, [20, 65, 1]
+    cache = Cache(rng, lens, 16, 2, 64, 64)
+    step = Step(rng, "bf16", [1] * 3, [n - 1 for n in lens])
+    tensors = {"q": step.q.contiguous(), "k": step.k.contiguous(), "v": step.v.contiguous(), "lengths": i32(lens), "table": torch.from_numpy(cache.table).cuda(),
+               **{n: cache.dev[n].clone() for n in ("k_codes", "k_scales", "v_codes", "v_scales")}, "history": step.rule_args[0], "spans": step.rule_args[1], "params": step.rule_args[2],
+               "masks": step.dev_masks, "out": step.out, "logits": step.logits}
+
+    def calls(r):
+        planes = [kc.NONE, r["lengths"], r["table"], r["k_codes"], r["k_scales"], r["v_codes"], r["v_scales"]]
+        return [kc.KernelCall.BlockCacheWrite(kc.BlockCacheWriteCall(r["k"], r["v"], *planes, rows, rows, 2, 64, 64, 128, 128, 16, cache.blocks, cache.width, kc.DTYPE_BF16)),
+                kc.KernelCall.BlockCacheAttention(kc.BlockCacheAttentionCall(r["q"], *planes, r["out"], rows, rows, 8, 2, 64, 64, 512, 512, 16, cache.blocks, cache.width, 0, kc.DTYPE_BF16)),
+                kc.KernelCall.LogitRules(kc.LogitRulesCall(r["out"], r["history"], r["spans"], r["params"], kc.NONE, kc.NONE, kc.NONE, r["masks"], kc.NONE, r["logits"], rows, 512, 512, 512,
+                                                           12, 0, rows, 16, kc.DTYPE_BF16))]
+
+    image = archive_of(calls, tensors, ("out", "logits"))
+    s = Slots(backend, 24)
+    for c in step.calls(s, cache, False):
+        backend.dispatch(c, s.ws)
+    backend.synchronize()
+    step.check(cache, False)
+    bits = lambda t: t.cpu().contiguous().view(torch.int16).numpy() if t.dtype == torch.bfloat16 else t.cpu().numpy()
+    session = hb.InferenceSession(backend, image)
+    for n, t in tensors.items():
+        if n not in ("out", "logits"):
+            session.write(n, bits(t))
+    session.execute()
+    assert np.array_equal(session.read("logits", np.int16).reshape(rows, 512), bits(step.logits))
+    session.capture()
+    session.execute()
+    assert np.array_equal(session.read("logits", np.int16).reshape(rows, 512), bits(step.logits))
+    assert np.array_equal(session.read("k_codes", np.int8).reshape(cache.host["k_codes"].shape), cache.host["k_codes"])
+    session.close()
+    with pytest.raises(hb.BackendError):
+        hb.InferenceSession(backend, image, addressed=True).close()
+
+
+def test_two_contexts_at_once():
+    """The same calls from two contexts on two streams, interleaved without waiting: each keeps to its own buffers."""
+    contexts = []
+    for seed in (31, 32):
+        be, stream, rng = hb.B200Backend(0), torch.cuda.Stream(), np.random.default_rng(seed)
+        be.set_stream(stream.cuda_stream)
+        few, many = Cache(rng, [2000, 700], 16, 2, 128, 128), Cache(rng, [1500, 900], 32, 2, 128, 128)
+        tensors = [strided(rng, 2, 1024, 1024, "bf16"), strided(rng, 300, 1024, 1024, "bf16"), strided(rng, 300, 256, 256, "bf16"), strided(rng, 300, 256, 256, "bf16")]
+        outs = [torch.zeros(n, 1024, dtype=torch.bfloat16, device="cuda") for n in (2, 300, 300)]
+        contexts.append((be, few, many, tensors, outs))
+
+    def run(be, few, many, t, outs):
+        return [attention(be, few, t[0], None, outs[0], 8, "bf16"), attention(be, many, t[1], [0, 180, 300], outs[1], 8, "bf16"),
+                packed(be, t[1], t[2], t[3], [0, 250, 300], outs[2], 8, 2, 128, 128, True, "bf16")]
+
+    wants = []
+    for c in contexts:
+        kept = run(*c)
+        c[0].synchronize()
+        wants.append([o.clone() for o in c[4]])
+        for o in c[4]:
+            o.zero_()
+    torch.cuda.synchronize()
+    slots = [run(*c) for c in contexts]          # binds once; what follows is only dispatched
+    del kept, slots
+    for _ in range(10):
+        kept = [run(*c) for c in contexts]
+    for c in contexts:
+        c[0].synchronize()
+    for c, want in zip(contexts, wants):
+        assert all(torch.equal(a, b) for a, b in zip(c[4], want))
+    for c in contexts:
+        c[0].close()
+
+
+@pytest.mark.parametrize("new,lens,block,heads,kv,dim,dtype", [
+    ([1] * 3, [3000, 40, 1700], 16, 8, 2, 128, "bf16"),
+    ([1] * 2, [3000, 1700], 32, 32, 2, 64, "f16"),
+    ([1] * 2, [5000, 1700], 32, 8, 2, 128, "f32"),
+    ([200, 90], [3000, 700], 16, 8, 2, 128, "bf16"),
+    ([200, 90], [3000, 700], 24, 8, 2, 128, "bf16"),
+    ([70, 90], [900, 700], 16, 8, 2, 64, "f32"),
+])
+def test_block_cache_attention_repeats_its_bits(backend, new, lens, block, heads, kv, dim, dtype):
+    """Parts of a sequence are joined in their order, whoever comes last."""
+    rng = np.random.default_rng(8)
+    cache, rows = Cache(rng, lens, block, kv, dim, dim), sum(new)
+    q = strided(rng, rows, heads * dim, heads * dim, dtype)
+    outs = [torch.zeros(rows, heads * dim, dtype=TORCH[dtype], device="cuda") for _ in range(6)]
+    for o in outs:
+        attention(backend, cache, q, starts_of(new), o, heads, dtype)
+    backend.synchronize()
+    assert all(torch.equal(outs[0], o) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_thousands_of_sequences(backend, dtype):
+    """More sequences than any table in shared memory has entries, most of them a token or none."""
+    rng = np.random.default_rng(9)
+    lens = rng.integers(0, 3, 5000)
+    lens[4000] = 150
+    starts, rows = starts_of(lens), int(lens.sum())
+    q, k, v = (strided(rng, rows, n * 64, n * 64, dtype) for n in (2, 1, 1))
+    out = torch.zeros(rows, 128, dtype=TORCH[dtype], device="cuda")
+    packed(backend, q, k, v, starts, out, 2, 1, 64, 64, True, dtype)
+    want, off = packed_reference(q, k, v, starts, 2, 1, 64, 64, True, dtype)
+    backend.synchronize()
+    check(f64(out), want, off)
+    # the same rows over a cache in which each sequence has up to 40 positions
+    have = [int(n) + int(rng.integers(0, 38)) if n else 0 for n in lens]
+    cache = Cache(rng, have, 16, 1, 64, 64)
+    out.zero_()
+    attention(backend, cache, q, starts, out, 2, dtype)
+    backend.synchronize()
+    got, qf = f64(out).reshape(rows, 2, 64), f64(q).reshape(rows, 2, 64)
+    for s in np.concatenate([rng.integers(0, 5000, 300), [0, 4000, 4999]]):
+        if lens[s]:
+            a, m, n = int(starts[s]), int(lens[s]), have[s]
+            kh, vh = cache.held("k", s, n)[:, 0], cache.held("v", s, n)[:, 0]
+            for h in range(2):
+                w, o = attend(qf[a:a + m, h], kh, vh, n - m + 1 + np.arange(m), 0.125, dtype, CACHE_WEIGHT_HALF[dtype])
+                check(got[a:a + m, h], w, o, f"sequence {s}")
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("dim", [128, 256])
+def test_a_cache_of_more_than_32_bits_of_bytes(backend, new, dim):
+    """The table names blocks on both sides of 2^31 and 2^32 bytes; the rest of the cache is never touched."""
+    rng = np.random.default_rng(10)
+    block, vdim = 1024, 16
+    blocks = 2 ** 32 // (block * dim) + 40
+    k_codes, v_codes = torch.empty(blocks, 1, block, dim, dtype=torch.int8, device="cuda"), torch.empty(blocks, 1, block, vdim, dtype=torch.int8, device="cuda")
+    scales = [torch.zeros(blocks, 1, device="cuda") for _ in range(2)]
+    named = [blocks - 1, 0, 2 ** 31 // (block * dim), 2 ** 32 // (block * dim)]
+    table = i32([named])
+    n = 3 * block + 77
+    k, v = strided(rng, n, dim, dim, "bf16"), strided(rng, n, vdim, vdim, "bf16")
+    s = Slots(backend)
+    planes = lambda starts, length: [s(i32(starts)), s(i32([length])), s(table), s(k_codes), s(scales[0]), s(v_codes), s(scales[1])]
+    backend.dispatch(kc.KernelCall.BlockCacheWrite(kc.BlockCacheWriteCall(s(k), s(v), *planes([0, n], n), n, 1, 1, dim, vdim, dim, vdim, block, blocks, 4, kc.DTYPE_BF16)), s.ws)
+    s = Slots(backend)
+    q, out = strided(rng, new, 2 * dim, 2 * dim, "bf16"), torch.zeros(new, 2 * vdim, dtype=torch.bfloat16, device="cuda")
+    backend.dispatch(kc.KernelCall.BlockCacheAttention(kc.BlockCacheAttentionCall(s(q), *planes([0, new], n), s(out), new, 1, 2, 1, dim, vdim, 2 * dim, 2 * vdim, block, blocks, 4, 0, kc.DTYPE_BF16)),
+                     s.ws)
+    backend.synchronize()
+    host = {"k": np.zeros((4, 1, block, dim), dtype=np.int8), "v": np.zeros((4, 1, block, vdim), dtype=np.int8)}
+    held = {}
+    for p, x, codes, scale in (("k", k, k_codes, scales[0]), ("v", v, v_codes, scales[1])):
+        want_scales = np.zeros((4, 1), dtype=np.float32)
+        write_plane(f64(x).reshape(n, 1, -1), host[p], want_scales, [0, n], [n], np.arange(4)[None], block)
+        at = torch.tensor(named, device="cuda")
+        assert np.array_equal(scale[at].cpu().numpy(), want_scales)
+        got = codes[at].cpu().numpy().reshape(4 * block, -1)[:n]
+        assert np.array_equal(got, host[p].reshape(4 * block, -1)[:n])
+        held[p] = got.astype(np.float64) * np.repeat(want_scales[:, 0].astype(np.float64), block)[:n, None]
+    got, qf = f64(out).reshape(new, 2, vdim), f64(q).reshape(new, 2, dim)
+    for h in range(2):
+        want, off = attend(qf[:, h], held["k"], held["v"], n - new + 1 + np.arange(new), dim ** -0.5, "bf16", CACHE_WEIGHT_HALF["bf16"])
+        check(got[:, h], want, off, f"head {h}")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_packed_rows_of_a_pitch_beyond_32_bits(backend, dtype):
+    """300 rows whose offsets pass 2^31 elements, k and v beside q in the same rows."""
+    rng = np.random.default_rng(13)
+    rows, pitch = 300, 8 * 10 ** 6
+    wide = torch.empty(rows * pitch, dtype=TORCH[dtype], device="cuda").view(rows, pitch)
+    wide[:, :256] = strided(rng, rows, 256, 256, dtype)
+    q, k, v = wide[:, :128], wide[:, 128:192], wide[:, 192:256]
+    out = torch.zeros(rows, 128, dtype=TORCH[dtype], device="cuda")
+    packed(backend, q, k, v, [0, 90, 300], out, 2, 1, 64, 64, True, dtype)
+    backend.synchronize()
+    want, off = packed_reference(q, k, v, [0, 90, 300], 2, 1, 64, 64, True, dtype)
+    check(f64(out), want, off)
+    del wide
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("new", [1, 60])
+def test_block_scales_far_apart_and_zero(backend, dtype, new):
+    """Value scales from 1 down to 2^-18 of the largest and none at all, key scales of zero; a block of each, and no block with a scale."""
+    rng = np.random.default_rng(14)
+    cache = Cache(rng, [16 * 19, 16 * 4, 80], 16, 1, 64, 64)
+    for j in range(19):
+        cache.host["v_scales"][cache.table[0, j]] = np.float32(2.0 ** -j / 127) if j % 5 else 0.0
+        cache.host["k_scales"][cache.table[0, j]] = 0.0 if j % 7 == 3 else np.float32(0.01)
+    for j in range(4):
+        cache.host["v_scales"][cache.table[1, j]] = 0.0
+    cache.dev = {n: torch.from_numpy(a.copy()).cuda() for n, a in cache.host.items()}
+    rows, starts = 3 * new, np.arange(4) * new
+    q, out = strided(rng, rows, 128, 128, dtype), torch.full((rows, 128), 7.0, dtype=TORCH[dtype], device="cuda")
+    attention(backend, cache, q, starts, out, 2, dtype)
+    backend.synchronize()
+    got, qf = f64(out).reshape(rows, 2, 64), f64(q).reshape(rows, 2, 64)
+    for s, n in enumerate(cache.lens):
+        k, v = cache.held("k", s, n)[:, 0], cache.held("v", s, n)[:, 0]
+        for h in range(2):
+            a = s * new
+            want, off = attend(qf[a:a + new, h], k, v, n - new + 1 + np.arange(new), 0.125, dtype, CACHE_WEIGHT_HALF[dtype])
+            check(got[a:a + new, h], want, off, f"sequence {s}")
