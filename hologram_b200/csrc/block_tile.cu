@@ -5,12 +5,12 @@
 //   warps 8-11 turn the tiles' codes into f16 (exact: integers of 8 bits) in the operands' swizzled layout, K and V through rings of two, a
 //              tile's codes on their way in registers while the one before is turned; and the query rows, scaled by a power of two to a largest
 //              value in [2^14, 2^15): exact in f16 but for values 2^29 smaller than the largest
-//   warp 1     tcgen05.mma issuer: S = Q K^T, then O += P V with P read from TMEM
+//   warp 1     tcgen05.mma issuer: S = Q K^T of a tile while the softmax of the one before runs, then O += P V with P read from TMEM
 //   warps 4-7  softmax, one thread per row. A block's scales are the same for 16 keys in a row: the key scale is a factor of the scores, the
 //              value scale a term of the exponent, w = 2^(s - max + log2 scale_v), and is taken out of the row's sum again. Weights are
 //              relative to a power of two above the largest value scale of the CTA's keys and rounded to f16 (2^-12 of a weight)
 // The tiles of all planes form one list that the CTAs share out evenly; parts of a plane are joined as for few rows (block_list.cuh).
-// Bound: one tile's chain scores -> softmax -> product; 128 rows leave the tensor core idle meanwhile. TMEM: S at 0, its weights over it, O at 128.
+// TMEM: S of even tiles at 0, of odd ones at 128, their weights over them, O at 256.
 #include "attention_issue.cuh"
 #include "block_list.cuh"
 
@@ -38,9 +38,9 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t* sm = smem_raw + (base - raw);
     const uint32_t k_bytes = p.k_chunks * TILE_CHUNK, v_bytes = p.v_chunks * TILE_CHUNK;
-    const uint32_t o_k = k_bytes, o_v = o_k + 2 * k_bytes, o_bars = o_v + 2 * v_bytes, bars = base + o_bars;
+    const uint32_t o_k = k_bytes, o_v = o_k + 2 * k_bytes, o_raw = o_v + 2 * v_bytes, raw_bytes = BT_TILE * (c.dim + c.vdim), o_bars = o_raw + 2 * raw_bytes, bars = base + o_bars;
     const uint32_t bar_q_full = bars, bar_q_empty = bars + 8, bar_k_full = bars + 16, bar_k_empty = bars + 32, bar_v_full = bars + 48, bar_v_empty = bars + 64,
-                   bar_s = bars + 80, bar_pa = bars + 88, bar_pb = bars + 96, bar_pv = bars + 104;
+                   bar_s = bars + 192, bar_pa = bars + 208, bar_pb = bars + 224;      // two of each, by tile: nobody is two phases of one ahead
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(sm + o_bars + 120);
     volatile uint32_t* s_abort = reinterpret_cast<volatile uint32_t*>(sm + o_bars + 124);
     uint32_t* s_last = reinterpret_cast<uint32_t*>(sm + o_bars + 128);
@@ -58,13 +58,12 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
             mbar_init(bar_k_empty + 8 * s, 1);
             mbar_init(bar_v_full + 8 * s, 4);
             mbar_init(bar_v_empty + 8 * s, 1);
+            mbar_init(bar_s + 8 * s, 2);      // the scores, and the issuer that has seen the tile's scales
+            mbar_init(bar_pa + 8 * s, 4);     // one arrival per softmax warp
+            mbar_init(bar_pb + 8 * s, 4);
         }
-        mbar_init(bar_s, 2);                  // the scores, and the issuer that has seen the tile's scales
         mbar_init(bar_workers, 4);
         mbar_init(bar_rows, 4);
-        mbar_init(bar_pa, 4);                 // one arrival per softmax warp
-        mbar_init(bar_pb, 4);
-        mbar_init(bar_pv, 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -73,7 +72,7 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
     Share mine;
     if (!find_share<BT_ROWS, BT_TILE, 2, 4>(c, group, &mine)) return;       // the same for every thread
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(256u) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -112,8 +111,10 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                 h[2 * e + 1] = codes_to_half<PICK23>(w[e]);
             }
             uint4* to = reinterpret_cast<uint4*>(tile + (unit >> 2) * TILE_CHUNK + key * 128);
-            to[(2 * (unit & 3u)) ^ (key & 7u)] = make_uint4(h[0], h[1], h[2], h[3]);
-            to[(2 * (unit & 3u) + 1) ^ (key & 7u)] = make_uint4(h[4], h[5], h[6], h[7]);
+            // the lanes of the two chunks begin with different halves: the eight lanes of a row meet all banks
+            const uint32_t late = unit >> 2, at = (2 * (unit & 3u) + late) ^ (key & 7u);
+            to[at] = late ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]);
+            to[at ^ 1u] = late ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(h[4], h[5], h[6], h[7]);
         };
         auto arrive = [&](uint32_t bar) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -139,40 +140,59 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                 }
                 return ((uint32_t)id * c.kv_heads + at.head) * br + (pos - block_of(pos) * br);
             };
-            uint4 kreg[8], vreg[8];
             float ks = 0.0f, vs = 0.0f;
-            auto load_codes = [&](uint4 (&to)[8], const int8_t* codes, uint32_t d, uint32_t from) {
+            // the codes of a tile into the ring, each unit by the thread that turns it
+            auto request = [&](uint32_t to, const int8_t* codes, uint32_t d, uint32_t from) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
+                for (uint32_t j = 0; j < 8; ++j) {
                     const uint32_t row = __shfl_sync(0xffffffffu, from, j);
-                    to[j] = row != 0xffffffffu && 16 * unit < d ? *reinterpret_cast<const uint4*>(codes + (uint64_t)(row + sub) * d + 16 * unit) : make_uint4(0, 0, 0, 0);
+                    const bool there = row != 0xffffffffu;
+                    if (16 * unit < d) cp_async16(base + to + (16 * j + sub) * d + 16 * unit, codes + (there ? (uint64_t)(row + sub) * d + 16 * unit : 0), there);
                 }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            auto turn_tile = [&](uint32_t to, uint32_t raw, uint32_t d) {
+                asm volatile("cp.async.wait_group 3;" ::: "memory");      // all but the last three requests
+                if (16 * unit < d)
+#pragma unroll 4
+                    for (uint32_t j = 0; j < 8; ++j) turn(sm + to, 16 * j + sub, *reinterpret_cast<const uint4*>(sm + raw + (16 * j + sub) * d + 16 * unit));
             };
             auto load_scales = [&](uint32_t from) {
                 const bool there = from != 0xffffffffu;
-                const uint32_t plane = there ? from / br : 0u;
+                const uint32_t plane = there ? block_of(from) : 0u;
                 ks = there ? c.k_scales[plane] : 0.0f;
                 vs = there ? c.v_scales[plane] : 0.0f;
             };
-            uint32_t from = rows_of(s0, find(s0));
-            int ahead = find(s0 + 1);
-            load_codes(kreg, c.k_codes, dim, from);
-            load_codes(vreg, c.v_codes, vdim, from);
+            const uint32_t raw_k[2] = {o_raw, o_raw + raw_bytes}, to_v = BT_TILE * dim;
+            asm volatile("cp.async.wait_group 0;" ::: "memory");      // what was requested behind the last plane's end
+            const int id0 = find(s0), id1 = find(s0 + 1);
+            int ahead = find(s0 + 2);
+            uint32_t from = rows_of(s0, id0);
             load_scales(from);
-            // this warp's query rows are on their way while the rest of the plane's beginning is done
-            const uint32_t row0 = (warp - 8) * 32;
-            const bool wide_q = ((uintptr_t)a.q & 7u) == 0 && (a.q_ld & 3u) == 0;
-            uint2 query[16];
-            auto load_query = [&](uint32_t r) {
-                const uint32_t flat = at.tile * BT_ROWS + r, i = flat / group;
-                const uint64_t q = (uint64_t)(at.first_row + i) * a.q_ld + (uint64_t)(at.head * group + flat - i * group) * dim + 4 * lane;
-                if (r >= rows || 4 * lane >= dim) return make_uint2(0, 0);
-                const uint16_t* from_q = (const uint16_t*)a.q + q;
-                if (wide_q) return *reinterpret_cast<const uint2*>(from_q);
-                return make_uint2(from_q[0] | (uint32_t)from_q[1] << 16, from_q[2] | (uint32_t)from_q[3] << 16);
-            };
+            request(raw_k[nt & 1u], c.k_codes, dim, from);
+            request(raw_k[nt & 1u] + to_v, c.v_codes, vdim, from);
+            from = rows_of(s0 + 1, id1);
+            request(raw_k[~nt & 1u], c.k_codes, dim, from);
+            request(raw_k[~nt & 1u] + to_v, c.v_codes, vdim, from);
+            // a thread its query row, on its way while the rest of the plane's beginning is done
+            uint4 query[16];
+            {
+                const uint32_t flat = at.tile * BT_ROWS + min(me, rows - 1), i = flat / group;
+                const uint16_t* from_q = (const uint16_t*)a.q + (uint64_t)(at.first_row + i) * a.q_ld + (uint64_t)(at.head * group + flat - i * group) * dim;
+                if (((uintptr_t)a.q & 15u) == 0 && (a.q_ld & 7u) == 0) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) query[r] = load_query(row0 + r);
+                    for (int u = 0; u < 16; ++u) query[u] = 8 * u < dim ? *reinterpret_cast<const uint4*>(from_q + 8 * u) : make_uint4(0, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) {
+                        uint32_t w[4] = {0, 0, 0, 0};
+                        if (8 * u < dim)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[e] = from_q[8 * u + 2 * e] | (uint32_t)from_q[8 * u + 2 * e + 1] << 16;
+                        query[u] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
             // the largest value scale of the CTA's part of the plane
             float largest = 0.0f;
             for (uint32_t b = block_of(s0 * BT_TILE) + me, last = block_of(min(s1 * BT_TILE, sees) - 1); b <= last; b += BT_WORKERS) {
@@ -190,39 +210,29 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
             const uint32_t top_bits = max(max(most_of[0], most_of[1]), max(most_of[2], most_of[3]));
             const int lift = max((int)(top_bits >> 23) - 126, -100);       // 2^lift is above it
             if (me == 0) s_lift[np & 1u] = lift;
-            // query rows, a warp a row at a time, four columns a lane: 16 lanes are a chunk of 64 columns, two lanes a unit
-#pragma unroll 1
-            for (uint32_t h = 0; h < 2; ++h) {
+            // magnitudes order as their bits do, infinities and NaN above all
+            uint32_t most = 0;
 #pragma unroll
-                for (int n = 0; n < 16; ++n) {
-                    const uint32_t r = row0 + 16 * h + n;
-                    const uint2 v = query[n];
-                    float x[4];
-                    if (a.dtype == HOLO_DTYPE_BF16) {
-                        x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
-                        x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
-                    } else {
-                        const float2 lo = half_values(v.x), hi = half_values(v.y);
-                        x[0] = lo.x; x[1] = lo.y; x[2] = hi.x; x[3] = hi.y;
-                    }
-                    // magnitudes order as their bits do, infinities and NaN above all
-                    uint32_t most = 0;
+            for (int u = 0; u < 16; ++u)
+                most = __vmaxu2(__vmaxu2(__vmaxu2(most, query[u].x & 0x7fff7fffu), query[u].y & 0x7fff7fffu), __vmaxu2(query[u].z & 0x7fff7fffu, query[u].w & 0x7fff7fffu));
+            most = max(most & 0xffffu, most >> 16);
+            most = __float_as_uint(a.dtype == HOLO_DTYPE_BF16 ? __uint_as_float(most << 16) : half_values(most).x);
+            const bool finite = most < 0x7f800000u;
+            // 2^e <= most < 2^(e + 1); two factors, since 2^(14 - e) alone may overflow
+            const int up = finite && most ? 14 - (most >> 23 ? (int)(most >> 23) - 127 : -118 - __clz((int)most)) : 0;
+            const float f0 = power_of_two(up / 2), f1 = power_of_two(up - up / 2);
+            const uint64_t first_factor = pair(f0, f0), second_factor = pair(f1, f1);
+            auto scaled = [&](uint32_t v) {
+                const float2 x = a.dtype == HOLO_DTYPE_BF16 ? make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)) : half_values(v);
+                const float2 y = unpair(mul2(mul2(pair(x.x, x.y), first_factor), second_factor));
+                return half_pair(y.x, y.y);
+            };
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
-                    most = __reduce_max_sync(0xffffffffu, most);
-                    const bool finite = most < 0x7f800000u;
-                    // 2^e <= most < 2^(e + 1); two factors, since 2^(14 - e) alone may overflow
-                    const int up = finite && most ? 14 - (most >> 23 ? (int)(most >> 23) - 127 : -118 - __clz((int)most)) : 0;
-                    const float f0 = power_of_two(up / 2), f1 = power_of_two(up - up / 2);
-                    if (4 * lane < dim)
-                        *reinterpret_cast<uint2*>(sm + (lane >> 4) * TILE_CHUNK + r * 128 + (((lane >> 1 & 7u) ^ (r & 7u)) << 4) + 8 * (lane & 1u)) =
-                            finite ? make_uint2(half_pair(x[0] * f0 * f1, x[1] * f0 * f1), half_pair(x[2] * f0 * f1, x[3] * f0 * f1)) : make_uint2(0, 0);
-                    if (lane == 0) s_row[(np & 1u) * BT_ROWS + r] = finite ? a.scale * LOG2E * power_of_two(-(up / 2)) * power_of_two(-(up - up / 2)) : NAN;
-                }
-                if (h == 0)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) query[r] = load_query(row0 + 16 + r);
-            }
+            for (int u = 0; u < 16; ++u)
+                if (8 * u < dim)
+                    *reinterpret_cast<uint4*>(sm + (u >> 3) * TILE_CHUNK + me * 128 + (((u & 7u) ^ (me & 7u)) << 4)) =
+                        finite ? make_uint4(scaled(query[u].x), scaled(query[u].y), scaled(query[u].z), scaled(query[u].w)) : make_uint4(0, 0, 0, 0);
+            s_row[(np & 1u) * BT_ROWS + me] = finite ? a.scale * LOG2E * power_of_two(-(up / 2)) * power_of_two(-(up - up / 2)) : NAN;
             arrive(bar_q_full);
             ++np;
 #pragma unroll 1
@@ -239,21 +249,17 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                 }
                 ok = nt < 2 || all_wait(bar_k_empty + 8 * stage, ((nt >> 1) - 1) & 1u);
                 if (!ok) break;
-                if (16 * unit < dim)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) turn(sm + o_k + stage * k_bytes, 16 * j + sub, kreg[j]);
+                turn_tile(o_k + stage * k_bytes, raw_k[stage], dim);
                 arrive(bar_k_full + 8 * stage);
-                from = rows_of(t + 1, ahead);
-                ahead = find(t + 2);
-                load_codes(kreg, c.k_codes, dim, from);
                 load_scales(from);
+                from = rows_of(t + 2, ahead);
+                ahead = find(t + 3);
+                request(raw_k[stage], c.k_codes, dim, from);
                 ok = nt < 2 || all_wait(bar_v_empty + 8 * stage, ((nt >> 1) - 1) & 1u);
                 if (!ok) break;
-                if (16 * unit < vdim)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) turn(sm + o_v + stage * v_bytes, 16 * j + sub, vreg[j]);
+                turn_tile(o_v + stage * v_bytes, raw_k[stage] + to_v, vdim);
                 arrive(bar_v_full + 8 * stage);
-                load_codes(vreg, c.v_codes, vdim, from);
+                request(raw_k[stage] + to_v, c.v_codes, vdim, from);
             }
         } while (ok && more(at));
     } else if (warp == 1) {
@@ -264,7 +270,7 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
         const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((vdim >> 3) << 17) | ((128u >> 4) << 24);
         const uint64_t first_q = smem_desc(uniform(base), 16, 1024), first_v = smem_desc(uniform(base + o_v), TILE_CHUNK, 1024);
         const uint32_t desc_q = (uint32_t)first_q, desc_k = (uint32_t)smem_desc(uniform(base + o_k), 16, 1024), high_s = (uint32_t)(first_q >> 32);
-        const uint32_t desc_v = (uint32_t)first_v, high_v = (uint32_t)(first_v >> 32), tmem_s = uniform(tmem_base), tmem_o = tmem_s + 128, ub = uniform(bars);
+        const uint32_t desc_v = (uint32_t)first_v, high_v = (uint32_t)(first_v >> 32), tmem_s = uniform(tmem_base), tmem_o = tmem_s + 256, ub = uniform(bars);
         const uint32_t ksteps = dim / 16;
         uint32_t nk = 0, nv = 0, np = 0;
         bool ok = true;
@@ -277,52 +283,49 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
             ok = wait(bar_q_full, np & 1u);
             ++np;
             for (uint32_t t = 0; t <= tiles && ok; ++t) {
-                // the product of key tile t - 1, the scores of key tile t
-                if (t < tiles) ok = wait(bar_k_full + 8 * (nk & 1u), (nk >> 1) & 1u);
-                if (ok && t > 0) {
-                    const uint32_t dv = desc_v + (nv & 1u) * (v_bytes >> 4), steps = min(8u, (keys - (t - 1) * 128 + 15) / 16);
-                    ok = wait(bar_v_full + 8 * (nv & 1u), (nv >> 1) & 1u) && wait(bar_pa, nv & 1u);
+                // the scores of key tile t, then the product of key tile t - 1, whose softmax runs meanwhile
+                if (t < tiles) {
+                    ok = wait(bar_k_full + 8 * (nk & 1u), (nk >> 1) & 1u);
                     if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) elected_ts(elected & (uint32_t)(k < steps), tmem_o, tmem_s + k * 8, dv + 128 * k, high_v, idesc_o, k | (t > 1));
-                    ok = wait(bar_pb, nv & 1u);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                    for (uint32_t k = 4; k < 8; ++k) elected_ts(elected & (uint32_t)(k < steps), tmem_o, tmem_s + k * 8, dv + 128 * k, high_v, idesc_o, 1);
-                    if (t == tiles) elected_commit(elected, ub + 104);
-                }
-                if (ok && t < tiles) {
-                    // the next scores go where the weights are, behind the product that reads them (see product_ss)
-                    const uint32_t dk = desc_k + (nk & 1u) * (k_bytes >> 4);
+                    // where the weights of tile t - 2 are, behind the product that reads them (see product_ss)
+                    const uint32_t dk = desc_k + (nk & 1u) * (k_bytes >> 4), to = tmem_s + 128 * (nk & 1u);
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                     for (uint32_t k = 0; k < 8; ++k) {
                         const uint32_t off = (k >> 2) * (TILE_CHUNK >> 4) + 2 * (k & 3u);
-                        elected_ss(elected & (uint32_t)(k < ksteps), tmem_s, desc_q + off, high_s, dk + off, high_s, idesc_s, k != 0);
+                        elected_ss(elected & (uint32_t)(k < ksteps), to, desc_q + off, high_s, dk + off, high_s, idesc_s, k != 0);
                     }
-                    elected_commit(elected, ub + 80);
-                    arrive_at(ub + 80);
+                    elected_commit(elected, ub + 192 + 8 * (nk & 1u));
+                    arrive_at(ub + 192 + 8 * (nk & 1u));
+                    elected_commit(elected, ub + 32 + 8 * (nk & 1u));
+                    if (t + 1 == tiles) elected_commit(elected, ub + 8);
+                    ++nk;
                 }
-                if (!ok) break;
                 if (t > 0) {
+                    const uint32_t dv = desc_v + (nv & 1u) * (v_bytes >> 4), steps = min(8u, (keys - (t - 1) * 128 + 15) / 16), weights = tmem_s + 128 * (nv & 1u);
+                    ok = wait(bar_v_full + 8 * (nv & 1u), (nv >> 1) & 1u) && wait(bar_pa + 8 * (nv & 1u), (nv >> 1) & 1u);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) elected_ts(elected & (uint32_t)(k < steps), tmem_o, weights + k * 8, dv + 128 * k, high_v, idesc_o, k | (t > 1));
+                    ok = wait(bar_pb + 8 * (nv & 1u), (nv >> 1) & 1u);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                    for (uint32_t k = 4; k < 8; ++k) elected_ts(elected & (uint32_t)(k < steps), tmem_o, weights + k * 8, dv + 128 * k, high_v, idesc_o, 1);
                     elected_commit(elected, ub + 64 + 8 * (nv & 1u));
                     ++nv;
-                }
-                if (t < tiles) {
-                    elected_commit(elected, ub + 32 + 8 * (nk & 1u));
-                    ++nk;
-                    if (t + 1 == tiles) elected_commit(elected, ub + 8);
                 }
             }
         } while (ok && more(at));
     } else if (warp >= 4) {
         // ---------------- softmax (TMEM lane quarter = warp % 4), then the output ----------------
         const uint32_t quarter = warp & 3u, lanes = (quarter * 32u) << 16, r = quarter * 32 + lane;
-        const uint32_t tmem_s = tmem_base + lanes, tmem_o = tmem_base + 128 + lanes;
+        const uint32_t tmem_first = tmem_base + lanes, tmem_o = tmem_base + 256 + lanes;
         uint32_t nt = 0, np = 0, met = 0;
         bool ok = true;
+        // the product of a tile is done (every phase of its barrier is waited for in turn)
+        auto product_of = [&](uint32_t tile) { return all_wait(bar_v_empty + 8 * (tile & 1u), (tile >> 1) & 1u); };
         Plane at = mine.first;
         do {
             uint32_t s0, s1;
@@ -333,8 +336,9 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
             // (the queries' barrier may be a plane ahead of this warp: what the workers left for the plane is read behind its first scores)
             float top = -INFINITY, sum = 0.0f, row_scale = 0.0f, back = 0.0f;
             for (uint32_t t = s0; t < s1; ++t, ++nt) {
-                ok = all_wait(bar_s, nt & 1u);
+                ok = all_wait(bar_s + 8 * (nt & 1u), (nt >> 1) & 1u) && (nt < 2 || product_of(nt - 2));
                 if (!ok) break;
+                const uint32_t tmem_s = tmem_first + 128 * (nt & 1u);
                 if (t == s0) {
                     row_scale = s_row[(np & 1u) * BT_ROWS + r];
                     back = power_of_two(s_lift[np & 1u] - BT_LIFT);
@@ -373,7 +377,10 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                     const float f = grows ? ex2(top - here) : 1.0f;      // 0 from the first scores on
                     if (grows) top = here;
                     sum *= f;
-                    if (t > s0) {    // the barrier of this tile's scores stands for the product before them too: O is at rest
+                    if (t > s0) {    // O is at rest when the product before is done; the next waits for this warp
+                        ok = product_of(nt - 1);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint64_t f2 = pair(f, f);
                         for (uint32_t x = 0; x < vdim; x += 16) {
                             uint32_t o[16];
@@ -414,12 +421,12 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(x == 1 ? bar_pa : bar_pb) : "memory");
+                        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"((x == 1 ? bar_pa : bar_pb) + 8 * (nt & 1u)) : "memory");
                     }
                 }
             }
             if (!ok) break;
-            ok = all_wait(bar_pv, np & 1u);
+            ok = product_of(nt - 1);
             ++np;
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -520,12 +527,12 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
     __syncthreads();
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(256u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
     }
 }
 
 int32_t launch_block_tile(holo_b200_ctx* ctx, const BlockTileParams& p) {
-    const uint32_t smem = 1024 + 3 * p.k_chunks * TILE_CHUNK + 2 * p.v_chunks * TILE_CHUNK + 256 + 2 * BT_ROWS * 4 + 4 * 24 * 4;
+    const uint32_t smem = 1024 + 3 * p.k_chunks * TILE_CHUNK + 2 * p.v_chunks * TILE_CHUNK + 2 * BT_TILE * (p.a.c.dim + p.a.c.vdim) + 256 + 2 * BT_ROWS * 4 + 4 * 24 * 4;
     static thread_local int configured_device = -1;
     if (configured_device != ctx->device) {
         HOLO_CUDA(cudaFuncSetAttribute(block_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ctx->smem_optin));
