@@ -2,9 +2,9 @@
 // 16 up to 128 and blocks of a multiple of 16 rows.
 //
 // A CTA takes 128 query rows of a kv head (a row is a new position and a head of the group) and walks the keys in tiles of 128:
-//   warps 8-11 turn the tiles' codes into f16 (exact: integers of 8 bits) in the operands' swizzled layout, K and V through rings of two, a
-//              tile's codes on their way in registers while the one before is turned; and the query rows, scaled by a power of two to a largest
-//              value in [2^14, 2^15): exact in f16 but for values 2^29 smaller than the largest
+//   warps 8-15 turn the tiles' codes into f16 (exact: integers of 8 bits) in the operands' swizzled layout, half of the warps K, half V, from
+//              rings of two that asynchronous copies fill into rings of two; and the query rows, scaled by a power of two to a largest value
+//              in [2^14, 2^15): exact in f16 but for values 2^29 smaller than the largest
 //   warp 1     tcgen05.mma issuer: S = Q K^T of a tile while the softmax of the one before runs, then O += P V with P read from TMEM
 //   warps 4-7  softmax, one thread per row. A block's scales are the same for 16 keys in a row: the key scale is a factor of the scores, the
 //              value scale a term of the exponent, w = 2^(s - max + log2 scale_v), and is taken out of the row's sum again. Weights are
@@ -16,7 +16,9 @@
 
 namespace {
 
-constexpr int BT_ROWS = 128, BT_TILE = 128, BT_WARPS = 12, BT_WORKERS = 128;      // threads that turn codes
+constexpr int BT_ROWS = 128, BT_TILE = 128, BT_WARPS = 16, BT_WORKERS = 128;      // threads that turn the codes of keys, and of values
+// registers a thread: the workers' and the issuer's leave what the softmax's 128 scores take (their sum is the launch's at most)
+constexpr int BT_ISSUER_REGS = 80, BT_SOFTMAX_REGS = 208, BT_WORKER_REGS = 112;
 constexpr float BT_GROWTH = 8.0f;
 constexpr int BT_LIFT = 7;
 
@@ -46,9 +48,9 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
     uint32_t* s_last = reinterpret_cast<uint32_t*>(sm + o_bars + 128);
     int* s_lift = reinterpret_cast<int*>(sm + o_bars + 132);                       // [2], by plane
     uint32_t* s_most = reinterpret_cast<uint32_t*>(sm + o_bars + 144);              // [2][4], by plane
-    const uint32_t bar_workers = bars + 176, bar_rows = bars + 184;                  // the four worker warps meet, the four softmax warps
+    const uint32_t bar_workers = bars + 176, bar_rows = bars + 184;                  // the eight worker warps meet, the four softmax warps
     float* s_row = reinterpret_cast<float*>(sm + o_bars + 256);                     // [2][128], by plane
-    float* s_scale = s_row + 2 * BT_ROWS;                                           // [4][3][8], by tile: key scales; exponents; reciprocals
+    float* s_scale = s_row + 2 * BT_ROWS;                                           // [8][3][8], by tile: key scales; exponents; reciprocals. The keys' workers are up to four tiles ahead of the softmax
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = p.group, dim = c.dim, vdim = c.vdim, br = c.block_rows;
     if (tid == 0) {
         mbar_init(bar_q_full, 4);             // one arrival per worker warp
@@ -62,7 +64,7 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
             mbar_init(bar_pa + 8 * s, 4);     // one arrival per softmax warp
             mbar_init(bar_pb + 8 * s, 4);
         }
-        mbar_init(bar_workers, 4);
+        mbar_init(bar_workers, 8);
         mbar_init(bar_rows, 4);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -95,9 +97,14 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
     auto all_wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, long_wait(bar, parity, s_abort, c.status)) != 0; };
 
     if (warp >= 8) {
-        // ---------------- workers: codes and queries into operands ----------------
+        // ---------------- workers: codes and queries into operands; warps 8-11 keys, 12-15 values ----------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BT_WORKER_REGS));
         // eight lanes take the 16-byte units of a row of codes, a warp four rows at a time: unit `unit` of keys 16 j + sub
-        const uint32_t me = tid - 8 * 32, unit = lane & 7u, sub = (warp - 8) * 4 + (lane >> 3);
+        const bool values = warp >= 12;
+        const uint32_t me = tid & 127u, unit = lane & 7u, sub = (warp & 3u) * 4 + (lane >> 3);
+        const int8_t* codes = values ? c.v_codes : c.k_codes;
+        const uint32_t d = values ? vdim : dim, raw0 = o_raw + (values ? 2 * BT_TILE * dim : 0u), raw_step = BT_TILE * d;
+        const uint32_t to0 = values ? o_v : o_k, to_step = values ? v_bytes : k_bytes, bar_full = values ? bar_v_full : bar_k_full, bar_empty = values ? bar_v_empty : bar_k_empty;
         uint32_t nt = 0, np = 0;
         bool ok = true;
         auto block_of = [&](uint32_t pos) { return p.br_shift >= 0 ? pos >> p.br_shift : pos / br; };
@@ -142,7 +149,7 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
             };
             float ks = 0.0f, vs = 0.0f;
             // the codes of a tile into the ring, each unit by the thread that turns it
-            auto request = [&](uint32_t to, const int8_t* codes, uint32_t d, uint32_t from) {
+            auto request = [&](uint32_t to, uint32_t from) {
 #pragma unroll
                 for (uint32_t j = 0; j < 8; ++j) {
                     const uint32_t row = __shfl_sync(0xffffffffu, from, j);
@@ -151,119 +158,119 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
-            auto turn_tile = [&](uint32_t to, uint32_t raw, uint32_t d) {
-                asm volatile("cp.async.wait_group 3;" ::: "memory");      // all but the last three requests
-                if (16 * unit < d)
-#pragma unroll 4
-                    for (uint32_t j = 0; j < 8; ++j) turn(sm + to, 16 * j + sub, *reinterpret_cast<const uint4*>(sm + raw + (16 * j + sub) * d + 16 * unit));
-            };
             auto load_scales = [&](uint32_t from) {
                 const bool there = from != 0xffffffffu;
                 const uint32_t plane = there ? block_of(from) : 0u;
                 ks = there ? c.k_scales[plane] : 0.0f;
                 vs = there ? c.v_scales[plane] : 0.0f;
             };
-            const uint32_t raw_k[2] = {o_raw, o_raw + raw_bytes}, to_v = BT_TILE * dim;
             asm volatile("cp.async.wait_group 0;" ::: "memory");      // what was requested behind the last plane's end
             const int id0 = find(s0), id1 = find(s0 + 1);
             int ahead = find(s0 + 2);
             uint32_t from = rows_of(s0, id0);
-            load_scales(from);
-            request(raw_k[nt & 1u], c.k_codes, dim, from);
-            request(raw_k[nt & 1u] + to_v, c.v_codes, vdim, from);
+            if (!values) load_scales(from);
+            request(raw0 + (nt & 1u) * raw_step, from);
             from = rows_of(s0 + 1, id1);
-            request(raw_k[~nt & 1u], c.k_codes, dim, from);
-            request(raw_k[~nt & 1u] + to_v, c.v_codes, vdim, from);
-            // a thread its query row, on its way while the rest of the plane's beginning is done
-            uint4 query[16];
-            {
-                const uint32_t flat = at.tile * BT_ROWS + min(me, rows - 1), i = flat / group;
-                const uint16_t* from_q = (const uint16_t*)a.q + (uint64_t)(at.first_row + i) * a.q_ld + (uint64_t)(at.head * group + flat - i * group) * dim;
-                if (((uintptr_t)a.q & 15u) == 0 && (a.q_ld & 7u) == 0) {
+            request(raw0 + (~nt & 1u) * raw_step, from);
+            volatile uint32_t* most_of = s_most + 4 * (np & 1u);
+            if (values) {
+                // the largest value scale of the CTA's part of the plane
+                float largest = 0.0f;
+                for (uint32_t b = block_of(s0 * BT_TILE) + me, last = block_of(min(s1 * BT_TILE, sees) - 1); b <= last; b += BT_WORKERS) {
+                    const int x = c.table[(uint64_t)at.seq * c.table_ld + b];
+                    const float f = (uint32_t)x < c.blocks ? c.v_scales[(uint64_t)x * c.kv_heads + at.head] : 0.0f;
+                    if (f < INFINITY) largest = fmaxf(largest, f);
+                }
+                const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
+                if (lane == 0) most_of[warp & 3u] = bits;
+            }
+            if (!values) {
+                // the queries' memory is free when the last plane's last scores are there
+                ok = np == 0 || all_wait(bar_q_empty, (np - 1) & 1u);
+                if (!ok) break;
+                // a thread its query row, on its way while the rest of the plane's beginning is done
+                uint4 query[16];
+                {
+                    const uint32_t flat = at.tile * BT_ROWS + min(me, rows - 1), i = flat / group;
+                    const uint16_t* from_q = (const uint16_t*)a.q + (uint64_t)(at.first_row + i) * a.q_ld + (uint64_t)(at.head * group + flat - i * group) * dim;
+                    if (((uintptr_t)a.q & 15u) == 0 && (a.q_ld & 7u) == 0) {
 #pragma unroll
-                    for (int u = 0; u < 16; ++u) query[u] = 8 * u < dim ? *reinterpret_cast<const uint4*>(from_q + 8 * u) : make_uint4(0, 0, 0, 0);
-                } else {
+                        for (int u = 0; u < 16; ++u) query[u] = 8 * u < dim ? *reinterpret_cast<const uint4*>(from_q + 8 * u) : make_uint4(0, 0, 0, 0);
+                    } else {
 #pragma unroll
-                    for (int u = 0; u < 16; ++u) {
-                        uint32_t w[4] = {0, 0, 0, 0};
-                        if (8 * u < dim)
+                        for (int u = 0; u < 16; ++u) {
+                            uint32_t w[4] = {0, 0, 0, 0};
+                            if (8 * u < dim)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = from_q[8 * u + 2 * e] | (uint32_t)from_q[8 * u + 2 * e + 1] << 16;
-                        query[u] = make_uint4(w[0], w[1], w[2], w[3]);
+                                for (int e = 0; e < 4; ++e) w[e] = from_q[8 * u + 2 * e] | (uint32_t)from_q[8 * u + 2 * e + 1] << 16;
+                            query[u] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
                     }
                 }
+                // magnitudes order as their bits do, infinities and NaN above all
+                uint32_t most = 0;
+#pragma unroll
+                for (int u = 0; u < 16; ++u)
+                    most = __vmaxu2(__vmaxu2(__vmaxu2(most, query[u].x & 0x7fff7fffu), query[u].y & 0x7fff7fffu), __vmaxu2(query[u].z & 0x7fff7fffu, query[u].w & 0x7fff7fffu));
+                most = max(most & 0xffffu, most >> 16);
+                most = __float_as_uint(a.dtype == HOLO_DTYPE_BF16 ? __uint_as_float(most << 16) : half_values(most).x);
+                const bool finite = most < 0x7f800000u;
+                // 2^e <= most < 2^(e + 1); two factors, since 2^(14 - e) alone may overflow
+                const int up = finite && most ? 14 - (most >> 23 ? (int)(most >> 23) - 127 : -118 - __clz((int)most)) : 0;
+                const float f0 = power_of_two(up / 2), f1 = power_of_two(up - up / 2);
+                const uint64_t first_factor = pair(f0, f0), second_factor = pair(f1, f1);
+                auto scaled = [&](uint32_t v) {
+                    const float2 x = a.dtype == HOLO_DTYPE_BF16 ? make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)) : half_values(v);
+                    const float2 y = unpair(mul2(mul2(pair(x.x, x.y), first_factor), second_factor));
+                    return half_pair(y.x, y.y);
+                };
+#pragma unroll
+                for (int u = 0; u < 16; ++u)
+                    if (8 * u < dim)
+                        *reinterpret_cast<uint4*>(sm + (u >> 3) * TILE_CHUNK + me * 128 + (((u & 7u) ^ (me & 7u)) << 4)) =
+                            finite ? make_uint4(scaled(query[u].x), scaled(query[u].y), scaled(query[u].z), scaled(query[u].w)) : make_uint4(0, 0, 0, 0);
+                s_row[(np & 1u) * BT_ROWS + me] = finite ? a.scale * LOG2E * power_of_two(-(up / 2)) * power_of_two(-(up - up / 2)) : NAN;
+                arrive(bar_q_full);
             }
-            // the largest value scale of the CTA's part of the plane
-            float largest = 0.0f;
-            for (uint32_t b = block_of(s0 * BT_TILE) + me, last = block_of(min(s1 * BT_TILE, sees) - 1); b <= last; b += BT_WORKERS) {
-                const int x = c.table[(uint64_t)at.seq * c.table_ld + b];
-                const float f = (uint32_t)x < c.blocks ? c.v_scales[(uint64_t)x * c.kv_heads + at.head] : 0.0f;
-                if (f < INFINITY) largest = fmaxf(largest, f);
-            }
-            const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
-            volatile uint32_t* most_of = s_most + 4 * (np & 1u);
-            if (lane == 0) most_of[warp - 8] = bits;
+            // all have what they keep of the plane before
             arrive_at(bar_workers);
-            // the queries' memory is free when the last plane's last scores are there
-            ok = (np == 0 || all_wait(bar_q_empty, (np - 1) & 1u)) && all_wait(bar_workers, np & 1u);
+            ok = all_wait(bar_workers, np & 1u);
             if (!ok) break;
             const uint32_t top_bits = max(max(most_of[0], most_of[1]), max(most_of[2], most_of[3]));
             const int lift = max((int)(top_bits >> 23) - 126, -100);       // 2^lift is above it
-            if (me == 0) s_lift[np & 1u] = lift;
-            // magnitudes order as their bits do, infinities and NaN above all
-            uint32_t most = 0;
-#pragma unroll
-            for (int u = 0; u < 16; ++u)
-                most = __vmaxu2(__vmaxu2(__vmaxu2(most, query[u].x & 0x7fff7fffu), query[u].y & 0x7fff7fffu), __vmaxu2(query[u].z & 0x7fff7fffu, query[u].w & 0x7fff7fffu));
-            most = max(most & 0xffffu, most >> 16);
-            most = __float_as_uint(a.dtype == HOLO_DTYPE_BF16 ? __uint_as_float(most << 16) : half_values(most).x);
-            const bool finite = most < 0x7f800000u;
-            // 2^e <= most < 2^(e + 1); two factors, since 2^(14 - e) alone may overflow
-            const int up = finite && most ? 14 - (most >> 23 ? (int)(most >> 23) - 127 : -118 - __clz((int)most)) : 0;
-            const float f0 = power_of_two(up / 2), f1 = power_of_two(up - up / 2);
-            const uint64_t first_factor = pair(f0, f0), second_factor = pair(f1, f1);
-            auto scaled = [&](uint32_t v) {
-                const float2 x = a.dtype == HOLO_DTYPE_BF16 ? make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)) : half_values(v);
-                const float2 y = unpair(mul2(mul2(pair(x.x, x.y), first_factor), second_factor));
-                return half_pair(y.x, y.y);
-            };
-#pragma unroll
-            for (int u = 0; u < 16; ++u)
-                if (8 * u < dim)
-                    *reinterpret_cast<uint4*>(sm + (u >> 3) * TILE_CHUNK + me * 128 + (((u & 7u) ^ (me & 7u)) << 4)) =
-                        finite ? make_uint4(scaled(query[u].x), scaled(query[u].y), scaled(query[u].z), scaled(query[u].w)) : make_uint4(0, 0, 0, 0);
-            s_row[(np & 1u) * BT_ROWS + me] = finite ? a.scale * LOG2E * power_of_two(-(up / 2)) * power_of_two(-(up - up / 2)) : NAN;
-            arrive(bar_q_full);
+            if (!values && me == 0) s_lift[np & 1u] = lift;
             ++np;
 #pragma unroll 1
             for (uint32_t t = s0; t < s1 && ok; ++t, ++nt) {
                 const uint32_t stage = nt & 1u;
                 // scales of 16 keys in a row, from the lane that has their block. A value scale 2^-60 of the largest and less is as good
                 // as none; its keys' weights still count in the rows' sums
-                if (me < 8) {
-                    float* to = s_scale + (nt & 3u) * 24 + me;
+                if (!values && me < 8) {
+                    float* to = s_scale + (nt & 7u) * 24 + me;
                     const float x = fmaxf(vs, power_of_two(max(lift - 60, -126)));
                     to[0] = ks;
                     to[8] = __log2f(x) + (float)(BT_LIFT - lift);
                     to[16] = __fdiv_rn(1.0f, x) * power_of_two(lift - BT_LIFT);
                 }
-                ok = nt < 2 || all_wait(bar_k_empty + 8 * stage, ((nt >> 1) - 1) & 1u);
+                ok = nt < 2 || all_wait(bar_empty + 8 * stage, ((nt >> 1) - 1) & 1u);
                 if (!ok) break;
-                turn_tile(o_k + stage * k_bytes, raw_k[stage], dim);
-                arrive(bar_k_full + 8 * stage);
-                load_scales(from);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");      // all but the last request
+                if (16 * unit < d) {
+                    uint8_t* to = sm + to0 + stage * to_step;
+                    const uint8_t* raw = sm + raw0 + stage * raw_step + 16 * unit;
+#pragma unroll 4
+                    for (uint32_t j = 0; j < 8; ++j) turn(to, 16 * j + sub, *reinterpret_cast<const uint4*>(raw + (16 * j + sub) * d));
+                }
+                arrive(bar_full + 8 * stage);
+                if (!values) load_scales(from);
                 from = rows_of(t + 2, ahead);
                 ahead = find(t + 3);
-                request(raw_k[stage], c.k_codes, dim, from);
-                ok = nt < 2 || all_wait(bar_v_empty + 8 * stage, ((nt >> 1) - 1) & 1u);
-                if (!ok) break;
-                turn_tile(o_v + stage * v_bytes, raw_k[stage] + to_v, vdim);
-                arrive(bar_v_full + 8 * stage);
-                request(raw_k[stage] + to_v, c.v_codes, vdim, from);
+                request(raw0 + stage * raw_step, from);
             }
         } while (ok && more(at));
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BT_ISSUER_REGS));
         const uint32_t elected = lane == 0;
         // D = f32, A and B f16, M = 128; S: both operands K-major, N = 128; O: V is N-major, N = vdim
         const uint32_t idesc_s = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
@@ -320,6 +327,7 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
         } while (ok && more(at));
     } else if (warp >= 4) {
         // ---------------- softmax (TMEM lane quarter = warp % 4), then the output ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BT_SOFTMAX_REGS));
         const uint32_t quarter = warp & 3u, lanes = (quarter * 32u) << 16, r = quarter * 32 + lane;
         const uint32_t tmem_first = tmem_base + lanes, tmem_o = tmem_base + 256 + lanes;
         uint32_t nt = 0, np = 0, met = 0;
@@ -348,7 +356,7 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                 uint32_t v[4][32];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) tmem_ld32_request(tmem_s + 32 * x, v[x]);
-                const float* scale = s_scale + (nt & 3u) * 24;
+                const float* scale = s_scale + (nt & 7u) * 24;
                 auto factor = [&](int g) { return fmaxf(row_scale * scale[g], 1e-37f); };      // above 0: -inf stays -inf
                 tmem_ld32_wait(v[0]);
 #pragma unroll
@@ -520,6 +528,8 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                 }
             }
         } while (more(at));
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BT_ISSUER_REGS));
     }
     // everyone meets here, whatever happened above, so that TMEM is always released
     __syncwarp();
@@ -532,7 +542,7 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
 }
 
 int32_t launch_block_tile(holo_b200_ctx* ctx, const BlockTileParams& p) {
-    const uint32_t smem = 1024 + 3 * p.k_chunks * TILE_CHUNK + 2 * p.v_chunks * TILE_CHUNK + 2 * BT_TILE * (p.a.c.dim + p.a.c.vdim) + 256 + 2 * BT_ROWS * 4 + 4 * 24 * 4;
+    const uint32_t smem = 1024 + 3 * p.k_chunks * TILE_CHUNK + 2 * p.v_chunks * TILE_CHUNK + 2 * BT_TILE * (p.a.c.dim + p.a.c.vdim) + 256 + 2 * BT_ROWS * 4 + 8 * 24 * 4;
     static thread_local int configured_device = -1;
     if (configured_device != ctx->device) {
         HOLO_CUDA(cudaFuncSetAttribute(block_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ctx->smem_optin));
