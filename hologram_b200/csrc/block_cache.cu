@@ -114,22 +114,35 @@ block_write_kernel(const __grid_constant__ HoloBlockWriteArgs a) {
     if (item == 0 && head == 0 && !values) check_sequences(c.starts, c.lengths, c.sequences, c.rows, most, c.status);
     // the sequence that owns the item, and the item's number in it
     uint32_t s, nth;
-    int64_t begin, count;
+    int64_t begin, count, length;
     if (c.starts) {
         // the last sequence whose first item is at most `item`: 32 places a round trip
         uint32_t lo = 0, left = c.sequences;
-        while (left > 0) {
+        int32_t from, to, has;
+        for (;;) {
             const uint32_t step = (left + 31) / 32, at = lo + min(tid & 31u, (left - 1) / step) * step;
-            const bool below = (int64_t)((uint32_t)max(c.starts[at], 0) / br) + 2ll * at <= (int64_t)item;
+            from = c.starts[at];
+            if (step == 1) {        // the last round: what is asked of the sequence comes along
+                to = c.starts[at + 1];
+                has = c.lengths[at];
+            }
+            const bool below = (int64_t)((uint32_t)max(from, 0) / br) + 2ll * at <= (int64_t)item;
             const uint32_t ahead = __ballot_sync(0xffffffffu, below);
             if (ahead == 0) return;         // starts that do not begin at 0
-            lo = __shfl_sync(0xffffffffu, at, 31 - __clz(ahead));
-            if (step == 1) break;
+            const int last = 31 - __clz(ahead);
+            lo = __shfl_sync(0xffffffffu, at, last);
+            if (step == 1) {
+                from = __shfl_sync(0xffffffffu, from, last);
+                to = __shfl_sync(0xffffffffu, to, last);
+                has = __shfl_sync(0xffffffffu, has, last);
+                break;
+            }
             left = min(step, c.sequences - lo);
         }
         s = lo;
-        begin = c.starts[s];
-        const int64_t end = c.starts[s + 1];
+        begin = from;
+        length = has;
+        const int64_t end = to;
         if (begin < 0 || end > c.rows) return;
         count = end - begin;
         nth = item - (uint32_t)begin / br - 2 * s;
@@ -138,39 +151,56 @@ block_write_kernel(const __grid_constant__ HoloBlockWriteArgs a) {
         begin = s;
         count = 1;
         nth = 0;
+        length = c.lengths[s];
     }
-    const int64_t length = c.lengths[s], first = length - count;
+    const int64_t first = length - count;
     if (count <= 0 || first < 0 || length > most) return;
     const uint32_t j = (uint32_t)first / br + nth, block_at = j * br;      // positions are below 2^31
     if ((int64_t)block_at >= length) return;
     const int id = c.table[(uint64_t)s * c.table_ld + j];
-    if (id < 0 || (uint32_t)id >= c.blocks) {
-        if (tid == 0) atomicOr(c.status, HOLO_STATUS_TABLE);
-        return;
-    }
     const uint32_t lo = first > block_at ? (uint32_t)first - block_at : 0u, hi = (uint32_t)min((int64_t)br, length - block_at);     // new rows of the block
     const uint32_t d = values ? c.vdim : c.dim, ld = values ? a.v_ld : a.k_ld;
-    const uint64_t plane = (uint64_t)id * c.kv_heads + head;
-    int8_t* codes = (values ? c.v_codes : c.k_codes) + plane * br * d;
-    float* scale = (values ? c.v_scales : c.k_scales) + plane;
     const void* x = values ? a.v : a.k;
     const uint64_t x0 = (uint64_t)(begin + (block_at + lo - first)) * ld + (uint64_t)head * d;      // the block's row `lo` in the call's rows
     const uint32_t across = d / VEC, n = (hi - lo) * across;
-    const float before = lo ? *scale : 0.0f;
     Unit<VEC> kept[WRITE_KEPT];
     auto unit = [&](uint32_t i) { return load_unit<DT, VEC>(x, x0 + (uint64_t)(i / across) * ld + (i % across) * VEC); };
 #pragma unroll
     for (int u = 0; u < WRITE_KEPT; ++u)
         if (tid + u * WRITE_THREADS < n) kept[u] = unit(tid + u * WRITE_THREADS);
+    // the rows are on their way while the block's number comes
+    if (id < 0 || (uint32_t)id >= c.blocks) {
+        if (tid == 0) atomicOr(c.status, HOLO_STATUS_TABLE);
+        return;
+    }
+    const uint64_t plane = (uint64_t)id * c.kv_heads + head;
+    int8_t* codes = (values ? c.v_codes : c.k_codes) + plane * br * d;
+    float* scale = (values ? c.v_scales : c.k_scales) + plane;
+    const float before = lo ? *scale : 0.0f;
     // magnitudes order as their bits do, infinities and NaN above all
     uint32_t largest = 0;
     auto look = [&](const Unit<VEC>& u, uint32_t below) {
-        float v[VEC];
-        values_of<DT, VEC>(u, v);
+        if constexpr (VEC == 8) {
+            // two 16-bit magnitudes at a time; what is not below becomes 0
+            const uint32_t w[4] = {u.raw.x & 0x7fff7fffu, u.raw.y & 0x7fff7fffu, u.raw.z & 0x7fff7fffu, u.raw.w & 0x7fff7fffu};
+            uint32_t m = 0;
+            if (below == 0xffffffffu) {
+                m = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
+            } else {
+                const uint32_t inf = DT == HOLO_DTYPE_BF16 ? 0x7f807f80u : 0x7c007c00u;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
-            if (m < below) largest = max(largest, m);
+                for (int e = 0; e < 4; ++e) m = __vmaxu2(m, w[e] & __vcmpltu2(w[e], inf));
+            }
+            m = max(m & 0xffffu, m >> 16);
+            largest = max(largest, DT == HOLO_DTYPE_BF16 ? m << 16 : __float_as_uint(__half2float(__ushort_as_half((uint16_t)m))));
+        } else {
+            float v[VEC];
+            values_of<DT, VEC>(u, v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const uint32_t m = __float_as_uint(v[e]) & 0x7fffffffu;
+                if (m < below) largest = max(largest, m);
+            }
         }
     };
     auto look_all = [&](uint32_t below) {
@@ -202,14 +232,16 @@ block_write_kernel(const __grid_constant__ HoloBlockWriteArgs a) {
         int code[VEC];
         bool special = !plain;
         if (plain) {
-            // |x / now| is 127 at most, but for roundings: a sum with 1.5 * 2^23 has the integer next to it in its low bits. The remainder
-            // is exact (see nearest_code); just half a step away it is left to that.
+            // |x / now| is 127 at most, but for roundings: a sum with 1.5 * 2^23 has the integer next to it in its low bits, and is it
+            // where the remainder (exact, see nearest_code) is below half a step; the few others are left to that
+            float most_left = 0.0f;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const float m = fmaf(v[e], inv, 12582912.0f), r = fmaf(12582912.0f - m, now, v[e]);
-                code[e] = __float_as_int(m) + (r > half ? 1 : 0) - (r < -half ? 1 : 0);
-                special = special || fabsf(r) == half;
+                code[e] = __float_as_int(m);
+                most_left = fmaxf(most_left, fabsf(r));
             }
+            special = most_left >= half;
         }
         if (special) {
 #pragma unroll
