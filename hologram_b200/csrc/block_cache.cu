@@ -34,6 +34,22 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
     return nearest_code(x, s, inv);
 }
 
+// Division of numbers below 2^31 by a number that the host knows, by a product: with 2^l >= d and m = floor(2^32 (2^l - d) / d) + 1,
+// n / d = (n + floor(m n / 2^32)) / 2^l (Granlund and Montgomery), where the sum fits 32 bits.
+struct Divisor {
+    uint32_t d, m, l;
+    explicit Divisor(uint32_t by) : d(by), l(0) {
+        while (1ull << l < by) ++l;
+        m = (uint32_t)((((1ull << l) - by) << 32) / by + 1);
+    }
+    __device__ __forceinline__ uint32_t of(uint32_t n) const { return (n + __umulhi(m, n)) >> l; }
+};
+struct BlockWriteParams {
+    HoloBlockWriteArgs a;
+    Divisor heads, block, k_across, v_across;      // across: units of a row
+    int32_t most;                                  // positions that a sequence may have
+};
+
 constexpr int WRITE_THREADS = 128;
 constexpr int WRITE_KEPT = 4;       // units of new values a thread keeps from the search for the largest to the coding
 
@@ -102,23 +118,23 @@ __device__ __noinline__ int any_code(float x, float s, float inv) { return code_
 // 128-thread CTAs, eight to an SM: what a CTA waits for is a chain of loads (starts, length, block number, rows), hidden by the others
 template <int DT, int VEC>
 __global__ void __launch_bounds__(WRITE_THREADS, 8)
-block_write_kernel(const __grid_constant__ HoloBlockWriteArgs a) {
+block_write_kernel(const __grid_constant__ BlockWriteParams p) {
     __shared__ uint32_t s_most[WRITE_THREADS / 32];
+    const HoloBlockWriteArgs& a = p.a;
     const HoloBlockCache& c = a.c;
     // neighbouring CTAs take the heads of the same rows, whose values lie side by side
-    const uint32_t head = blockIdx.x % c.kv_heads, item = blockIdx.x / c.kv_heads >> 1, tid = threadIdx.x, br = c.block_rows;
-    const bool values = (blockIdx.x / c.kv_heads & 1u) != 0;
+    const uint32_t turn = p.heads.of(blockIdx.x), head = blockIdx.x - turn * c.kv_heads, item = turn >> 1, tid = threadIdx.x, br = c.block_rows;
+    const bool values = (turn & 1u) != 0;
     holo_pdl_trigger();
     holo_pdl_wait();
-    const int64_t most = (int64_t)c.table_ld * br;
-    if (item == 0 && head == 0 && !values) check_sequences(c.starts, c.lengths, c.sequences, c.rows, most, c.status);
+    if (blockIdx.x == 0) check_sequences(c.starts, c.lengths, c.sequences, c.rows, p.most, c.status);
     // the sequence that owns the item, and the item's number in it
     uint32_t s, nth;
-    int64_t begin, count, length;
+    int32_t begin, end, length;
     if (c.starts) {
         // the last sequence whose first item is at most `item`: 32 places a round trip
         uint32_t lo = 0, left = c.sequences;
-        int32_t from, to, has;
+        int32_t from, to = 0, has = 0;
         for (;;) {
             const uint32_t step = (left + 31) / 32, at = lo + min(tid & 31u, (left - 1) / step) * step;
             from = c.starts[at];
@@ -126,7 +142,7 @@ block_write_kernel(const __grid_constant__ HoloBlockWriteArgs a) {
                 to = c.starts[at + 1];
                 has = c.lengths[at];
             }
-            const bool below = (int64_t)((uint32_t)max(from, 0) / br) + 2ll * at <= (int64_t)item;
+            const bool below = (uint64_t)p.block.of((uint32_t)max(from, 0)) + 2ull * at <= item;
             const uint32_t ahead = __ballot_sync(0xffffffffu, below);
             if (ahead == 0) return;         // starts that do not begin at 0
             const int last = 31 - __clz(ahead);
@@ -141,30 +157,33 @@ block_write_kernel(const __grid_constant__ HoloBlockWriteArgs a) {
         }
         s = lo;
         begin = from;
+        end = to;
         length = has;
-        const int64_t end = to;
-        if (begin < 0 || end > c.rows) return;
-        count = end - begin;
-        nth = item - (uint32_t)begin / br - 2 * s;
+        if (begin < 0 || end <= begin || end > (int32_t)c.rows) return;
+        nth = item - p.block.of((uint32_t)begin) - 2 * s;
     } else {
         s = item;
-        begin = s;
-        count = 1;
+        begin = (int32_t)s;
+        end = begin + 1;
         nth = 0;
         length = c.lengths[s];
     }
-    const int64_t first = length - count;
-    if (count <= 0 || first < 0 || length > most) return;
-    const uint32_t j = (uint32_t)first / br + nth, block_at = j * br;      // positions are below 2^31
-    if ((int64_t)block_at >= length) return;
+    const int32_t count = end - begin;
+    if (length < count || length > p.most || nth > p.block.of((uint32_t)count - 1) + 1) return;
+    const uint32_t first = (uint32_t)(length - count), j = p.block.of(first) + nth, block_at = j * br;      // positions are below 2^31
+    if (block_at >= (uint32_t)length) return;
     const int id = c.table[(uint64_t)s * c.table_ld + j];
-    const uint32_t lo = first > block_at ? (uint32_t)first - block_at : 0u, hi = (uint32_t)min((int64_t)br, length - block_at);     // new rows of the block
+    const uint32_t lo = first > block_at ? first - block_at : 0u, hi = min(br, (uint32_t)length - block_at);     // new rows of the block
     const uint32_t d = values ? c.vdim : c.dim, ld = values ? a.v_ld : a.k_ld;
     const void* x = values ? a.v : a.k;
-    const uint64_t x0 = (uint64_t)(begin + (block_at + lo - first)) * ld + (uint64_t)head * d;      // the block's row `lo` in the call's rows
-    const uint32_t across = d / VEC, n = (hi - lo) * across;
+    const uint64_t x0 = (uint64_t)((uint32_t)begin + (block_at + lo - first)) * ld + (uint64_t)head * d;      // the block's row `lo` in the call's rows
+    const Divisor& units = values ? p.v_across : p.k_across;
+    const uint32_t across = units.d, n = (hi - lo) * across;
     Unit<VEC> kept[WRITE_KEPT];
-    auto unit = [&](uint32_t i) { return load_unit<DT, VEC>(x, x0 + (uint64_t)(i / across) * ld + (i % across) * VEC); };
+    auto unit = [&](uint32_t i) {
+        const uint32_t row = units.of(i);
+        return load_unit<DT, VEC>(x, x0 + (uint64_t)row * ld + (i - row * across) * VEC);
+    };
 #pragma unroll
     for (int u = 0; u < WRITE_KEPT; ++u)
         if (tid + u * WRITE_THREADS < n) kept[u] = unit(tid + u * WRITE_THREADS);
@@ -307,7 +326,9 @@ int32_t holo_launch_block_cache_write(holo_b200_ctx* ctx, const HoloBlockWriteAr
     const uint32_t es = (uint32_t)holo_dtype_size(a.dtype), vec = 16 / es;
     const bool wide = ((((uintptr_t)a.k | (uintptr_t)a.v) & 15u) | (a.c.dim | a.c.vdim | a.k_ld | a.v_ld) % vec) == 0 && (((uintptr_t)a.c.k_codes | (uintptr_t)a.c.v_codes) & 7u) == 0;
     const dim3 grid((uint32_t)(items * a.c.kv_heads * 2)), block(WRITE_THREADS);
-    auto launch = [&](auto kernel) { return holo_launch_kernel(ctx, kernel, grid, block, 0, 1, a); };
+    const uint32_t per = wide ? vec : 1u;
+    const BlockWriteParams p = {a, Divisor(a.c.kv_heads), Divisor(a.c.block_rows), Divisor(a.c.dim / per), Divisor(a.c.vdim / per), (int32_t)(a.c.table_ld * a.c.block_rows)};
+    auto launch = [&](auto kernel) { return holo_launch_kernel(ctx, kernel, grid, block, 0, 1, p); };
     cudaError_t e;
     if (a.dtype == HOLO_DTYPE_F32) e = wide ? launch(block_write_kernel<HOLO_DTYPE_F32, 4>) : launch(block_write_kernel<HOLO_DTYPE_F32, 1>);
     else if (a.dtype == HOLO_DTYPE_BF16) e = wide ? launch(block_write_kernel<HOLO_DTYPE_BF16, 8>) : launch(block_write_kernel<HOLO_DTYPE_BF16, 1>);

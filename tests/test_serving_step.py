@@ -80,6 +80,19 @@ def test_nearest_codes_in_32_bits():
         assert np.array_equal(np.clip(n, -127, 127).astype(np.int8), encode(y, scale))
 
 
+def test_division_by_a_product():
+    """n // d for n below 2^31 as (n + (m n >> 32)) >> l with 2^l >= d, m = (2^l - d) 2^32 // d + 1, all of 32 bits."""
+    rng = np.random.default_rng(3)
+    for d in [1, 2, 3, 5, 7, 8, 10, 12, 16, 24, 33, 48, 63, 64, 65, 100, 127, 128, 255, 257, 512, 513, 1000, 1023, 1024, 65535, 2 ** 20 + 1, 2 ** 31 - 1]:
+        l = (d - 1).bit_length()
+        m = ((2 ** l - d) << 32) // d + 1
+        assert m < 2 ** 32
+        for n in [0, 1, d - 1, d, d + 1, 2 * d - 1, 2 * d, 2 ** 31 - 1, 2 ** 31 - 2, (2 ** 31 - 1) // d * d, (2 ** 31 - 1) // d * d - 1] + rng.integers(0, 2 ** 31, 500).tolist():
+            if n < 2 ** 31:
+                high = m * n >> 32
+                assert n + high < 2 ** 32 and (n + high) >> l == n // d
+
+
 def test_every_touched_block_is_one_item_of_the_write():
     """Sequence s owns items starts[s] / block + 2 s and on; no two sequences share one and none runs out of them."""
     rng = np.random.default_rng(1)
