@@ -72,7 +72,7 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
     holo_pdl_wait();
     if (blockIdx.x == 0) check_sequences(c.starts, c.lengths, c.sequences, c.rows, (int64_t)c.table_ld * br, c.status);
     Share mine;
-    if (!find_share<BT_ROWS, BT_TILE, 2, 4>(c, group, &mine)) return;       // the same for every thread
+    if (!find_share<BT_ROWS, BT_TILE, 4, 4>(c, group, &mine)) return;       // the same for every thread
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -496,33 +496,45 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
                 ok = all_wait(bar_rows, met++ & 1u);
                 if (!ok) break;
                 if (*reinterpret_cast<volatile uint32_t*>(s_last)) {
-                    // a thread its row
+                    // A thread the weights of its row's parts, which take the place of their maxima; then the four warps take 16 columns of
+                    // 32 rows in turn, four parts' values on their way at a time
                     const uint32_t step = 2 * BT_ROWS * (vdim + 2), own = BT_ROWS * (vdim + 2);
-                    const float* first = p.partials + (uint64_t)from_cta * step + r;
+                    float* const first = p.partials + (uint64_t)from_cta * step;
                     auto part = [&](uint32_t w) { return first + (uint64_t)w * step + (w == 0 ? own : 0u); };
                     if (r < rows) {
                         float m = -INFINITY, l = 0.0f;
-#pragma unroll 4
-                        for (uint32_t w = 0; w < count; ++w) m = fmaxf(m, __ldcg(part(w) + vdim * BT_ROWS));
-                        auto weight = [&](uint32_t w, float sum_w) { return sum_w == 0.0f ? 0.0f : ex2(__ldcg(part(w) + vdim * BT_ROWS) - m); };      // NaN is not 0
+#pragma unroll 8
+                        for (uint32_t w = 0; w < count; ++w) m = fmaxf(m, __ldcg(part(w) + vdim * BT_ROWS + r));
 #pragma unroll 4
                         for (uint32_t w = 0; w < count; ++w) {
-                            const float lw = __ldcg(part(w) + (vdim + 1) * BT_ROWS);
-                            l = fmaf(weight(w, lw), lw, l);
+                            float* const of = part(w) + vdim * BT_ROWS + r;
+                            const float lw = __ldcg(of + BT_ROWS), f = lw == 0.0f ? 0.0f : ex2(__ldcg(of) - m);      // NaN is not 0
+                            l = fmaf(f, lw, l);
+                            __stcg(of, f);
                         }
-                        const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-                        for (uint32_t x = 0; x < vdim; x += 16) {
-                            float acc[16];
+                        __stcg(part(0) + (vdim + 1) * BT_ROWS + r, l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l));
+                    }
+                    arrive_at(bar_rows);
+                    ok = all_wait(bar_rows, met++ & 1u);
+                    if (!ok) break;
+                    const uint32_t chunks = vdim / 16, tasks = (rows + 31) / 32 * chunks;
+#pragma unroll 1
+                    for (uint32_t task = quarter; task < tasks; task += 4) {
+                        const uint32_t row = task / chunks * 32 + lane, x = task % chunks * 16;
+                        if (row >= rows) continue;
+                        float acc[16];
 #pragma unroll
-                            for (int y = 0; y < 16; ++y) acc[y] = 0.0f;
-#pragma unroll 2
-                            for (uint32_t w = 0; w < count; ++w) {
-                                const float f = weight(w, __ldcg(part(w) + (vdim + 1) * BT_ROWS)) * inv;
+                        for (int y = 0; y < 16; ++y) acc[y] = 0.0f;
+#pragma unroll 4
+                        for (uint32_t w = 0; w < count; ++w) {
+                            const float *from = part(w) + row, f = __ldcg(from + vdim * BT_ROWS);
 #pragma unroll
-                                for (int y = 0; y < 16; ++y) acc[y] = fmaf(f, __ldcg(part(w) + (x + y) * BT_ROWS), acc[y]);
-                            }
-                            store16(out + x, acc);
+                            for (int y = 0; y < 16; ++y) acc[y] = fmaf(f, __ldcg(from + (x + y) * BT_ROWS), acc[y]);
                         }
+                        const float inv = __ldcg(part(0) + (vdim + 1) * BT_ROWS + row);
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) acc[y] *= inv;
+                        store16(out_of(row) + x, acc);
                     }
                     __syncwarp();
                 }
@@ -561,8 +573,9 @@ int32_t holo_try_block_tile(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool
     const uint32_t group = a.heads / c.kv_heads;
     if (a.dtype == HOLO_DTYPE_F32 || c.block_rows % 16 != 0) return HOLO_OK;
     if (c.dim % 16 != 0 || c.vdim % 16 != 0 || c.dim > 128 || c.vdim > 128 || (((uintptr_t)c.k_codes | (uintptr_t)c.v_codes) & 15u) != 0) return HOLO_OK;
-    // where a sequence has more rows of a head than the few-row kernel takes in three passes over the cache
-    if ((uint64_t)c.rows * group <= 24ull * c.sequences) return HOLO_OK;
+    // where a sequence has more rows of a head than the few-row kernel takes in two passes over the cache: three take 78 us against 56 here for
+    // 8 sequences of 4096 positions (137 against 101 for 32 of 2048, 28 against 28 for one of 4096), two 63 (101, 22)
+    if ((uint64_t)c.rows * group <= 16ull * c.sequences) return HOLO_OK;
     // tiles of the whole list of 32 bits
     const uint64_t tiles = ((uint64_t)c.rows * group / BT_ROWS + c.sequences) * c.kv_heads;
     if ((uint64_t)c.rows * a.heads > 0x7fffffffull || tiles > 0x7fffffffull / (((uint64_t)c.table_ld * c.block_rows + BT_TILE - 1) / BT_TILE)) return HOLO_OK;
