@@ -15,6 +15,7 @@ constexpr int RULES_THREADS = 256;
 constexpr int RULES_KEPT = 4;                 // units of logits a thread requests before the counts are there
 constexpr int RULES_AHEAD = 8;                // history entries a thread has on their way
 constexpr uint32_t RULES_MOST_PART = 8192;    // tokens of a CTA: counts and bias entries are 8 bytes a token
+constexpr uint32_t RULES_MOST_Y = 65535;      // rows of a grid's second dimension; more go on in the third
 constexpr uint32_t IN_PROMPT = 0x80000000u;   // of a count: the token stands in the prompt; the rest counts it behind the prompt
 
 struct RulesParams {
@@ -36,9 +37,10 @@ __global__ void __launch_bounds__(RULES_THREADS)
 logit_rules_kernel(const __grid_constant__ RulesParams p) {
     extern __shared__ __align__(16) uint32_t s_words[];     // counts [part], then bias entries + 1 [part]
     const HoloLogitRulesArgs& a = p.a;
-    const uint32_t tid = threadIdx.x, row = blockIdx.y, first = blockIdx.x * p.part, n = min(p.part, a.vocab - first);
+    const uint32_t tid = threadIdx.x, row = blockIdx.z * gridDim.y + blockIdx.y, first = blockIdx.x * p.part, n = min(p.part, a.vocab - first);
     holo_pdl_trigger();
     holo_pdl_wait();
+    if (row >= a.rows) return;
     // what this thread's first logits are: on their way while the history is counted
     const uint64_t z0 = (uint64_t)row * a.ld + first, o0 = (uint64_t)row * a.out_ld + first;
     RulesUnit<VEC> kept[RULES_KEPT];
@@ -172,7 +174,7 @@ int32_t launch_logit_rules(holo_b200_ctx* ctx, const RulesParams& p) {
         HOLO_CUDA(cudaFuncSetAttribute(logit_rules_kernel<DT, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(RULES_MOST_PART * 8)));
         configured_device = ctx->device;
     }
-    HOLO_CUDA(holo_launch_kernel(ctx, logit_rules_kernel<DT, VEC>, dim3((p.a.vocab + p.part - 1) / p.part, p.a.rows), dim3(RULES_THREADS), smem, 1, p));
+    HOLO_CUDA(holo_launch_kernel(ctx, logit_rules_kernel<DT, VEC>, dim3((p.a.vocab + p.part - 1) / p.part, p.a.rows < RULES_MOST_Y ? p.a.rows : RULES_MOST_Y, (p.a.rows + RULES_MOST_Y - 1) / RULES_MOST_Y), dim3(RULES_THREADS), smem, 1, p));
     ctx->launches++;
     return HOLO_OK;
 }
@@ -180,7 +182,6 @@ int32_t launch_logit_rules(holo_b200_ctx* ctx, const RulesParams& p) {
 }  // namespace
 
 int32_t holo_launch_logit_rules(holo_b200_ctx* ctx, const HoloLogitRulesArgs& a) {
-    if (a.rows > 65535) return holo_fail(HOLO_ERR_UNSUPPORTED_OP, "unsupported op: logit_rules of %u rows", a.rows);
     RulesParams p = {};
     p.a = a;
     const uint32_t es = (uint32_t)holo_dtype_size(a.dtype), vec = 16 / es;

@@ -584,6 +584,20 @@ def test_logit_rules_each_alone(backend):
     assert np.array_equal(f64(out), zf)
 
 
+def test_logit_rules_of_more_rows_than_a_grid_is_high(backend):
+    rng = np.random.default_rng(15)
+    z = strided(rng, 70000, 33, 33, "f32")
+    out = torch.zeros(70000, 33, device="cuda")
+    history = torch.from_numpy(rng.integers(0, 33, (70000, 3)).astype(np.int32)).cuda()
+    apply_rules(backend, z, out, history, i32([[0, 3]]).repeat(70000, 1), torch.tensor([[1.0, 0.5, 0.0, 0.0]], device="cuda").repeat(70000, 1))
+    backend.synchronize()
+    want = f64(z)
+    seen = np.zeros((70000, 33), dtype=bool)
+    np.put_along_axis(seen, history.cpu().numpy(), True, 1)
+    # a difference with 0.5 in f32: one rounding of a value
+    assert np.all(np.abs(f64(out) - (want - 0.5 * seen)) <= 2.0 ** -24 * (np.abs(want) + 0.5))
+
+
 @pytest.mark.parametrize("what", ["spans", "total", "bias", "mask"])
 def test_logit_rules_report_bad_numbers(backend, what):
     z, out = torch.zeros(2, 100, device="cuda"), torch.zeros(2, 100, device="cuda")
