@@ -145,7 +145,7 @@ static int32_t check_dev_status(holo_b200_ctx* ctx, void* host = nullptr, const 
     }
     if (st == 0) return HOLO_OK;
     cudaMemsetAsync(ctx->dev_status, 0, 4, ctx->stream);
-    if (st & 2u) cudaMemsetAsync(ctx->attn_arrivals, 0, 65536 * 4, ctx->stream);  // a launch that gave up may have left counts behind
+    if (st & 6u) cudaMemsetAsync(ctx->attn_arrivals, 0, 65536 * 4, ctx->stream);  // a launch that gave up may have left counts behind
     if (st & 1u) return holo_fail_slot(HOLO_NO_SLOT, "gather index outside [−axis_dim, axis_dim)");
     if (st & HOLO_STATUS_TABLE)
         return holo_fail(HOLO_ERR_DISPATCH, "dispatch failed: a call's starts, lengths, block numbers, spans or mask numbers on the device are out of range (status 0x%x)", st);

@@ -454,7 +454,7 @@ struct HoloLogitRulesArgs {
 };
 int32_t holo_launch_logit_rules(holo_b200_ctx* ctx, const HoloLogitRulesArgs& a);
 // bits of the status word: what a kernel found out of range on the device
-constexpr uint32_t HOLO_STATUS_TABLE = 8u;
+constexpr uint32_t HOLO_STATUS_TABLE = 256u;      // 1 to 16: indexes of gather, waits that gave up, zero points
 // quant_gemv.cu
 int32_t holo_launch_matmul_e8cb_omajor(holo_b200_ctx* ctx, const float* a, const uint8_t* bq, const int8_t* codebook, const float* scales,
                                        const int32_t* zero_points, const float* residual, float* out, uint32_t m, uint32_t k, uint32_t n, int act);

@@ -80,6 +80,18 @@ def test_nearest_codes_in_32_bits():
         assert np.array_equal(np.clip(n, -127, 127).astype(np.int8), encode(y, scale))
 
 
+def test_the_status_of_bad_tables_is_no_other_failure_s():
+    import re
+    folder = os.path.join(ROOT, "hologram_b200", "csrc")
+    used, own = set(), None
+    for name in os.listdir(folder):
+        if name.endswith((".cu", ".cuh", ".h", ".cpp")):
+            text = open(os.path.join(folder, name)).read()
+            used |= {int(n) for n in re.findall(r"atomicOr\([^;]*?status, (\d+)u\)", text)}
+            own = next((int(n) for n in re.findall(r"HOLO_STATUS_TABLE = (\d+)u", text)), own)
+    assert {1, 2, 4, 8} <= used and own and not any(own & n for n in used)
+
+
 def test_division_by_a_product():
     """n // d for n below 2^31 as (n + (m n >> 32)) >> l with 2^l >= d, m = (2^l - d) 2^32 // d + 1, all of 32 bits."""
     rng = np.random.default_rng(3)
