@@ -64,10 +64,11 @@ __device__ __forceinline__ void read_sequence(const HoloBlockCache& c, uint32_t 
     p->tiles = (p->n * group + R - 1) / R;
     p->head = p->tile = 0;
 }
-// On to the next plane that has slabs; slabs == 0: there is none.
-template <int R, int SLAB>
+// On to the next plane that has slabs; slabs == 0: there is none. EXTRA: places of the list behind a plane's slabs that stand for what a
+// plane costs a CTA beside them.
+template <int R, int SLAB, int EXTRA = 0>
 __device__ __forceinline__ void next_plane(const HoloBlockCache& c, uint32_t group, Plane* p) {
-    p->at += p->slabs;
+    p->at += p->slabs + EXTRA;
     for (;;) {
         if (++p->tile >= p->tiles) {
             p->tile = 0;
@@ -109,10 +110,10 @@ struct Share {
 // Every warp finds the share by itself, four sequences a lane at a time; false: there is none for this CTA. A share is LEAST slabs at
 // least, so that fewer CTAs take part in a short list. Planes are cut apart where that lengthens a share by less than the SECOND
 // slabs that another plane costs a CTA.
-template <int R, int SLAB, int LEAST, int SECOND>
+template <int R, int SLAB, int LEAST, int SECOND, int EXTRA = 0>
 __device__ __forceinline__ bool find_share(const HoloBlockCache& c, uint32_t group, Share* out) {
     const uint32_t lane = threadIdx.x & 31;
-    uint32_t cnt[4], upto = 0, sum = 0, all = 0, planes = 0, unit = 1;
+    uint32_t cnt[4], upto = 0, sum = 0, all = 0, planes = 0, unit = 1, extra = 0;
     auto count_chunk = [&](uint32_t s0) {
         Plane seq[4];
 #pragma unroll
@@ -126,7 +127,10 @@ __device__ __forceinline__ bool find_share(const HoloBlockCache& c, uint32_t gro
         for (int i = 0; i < 4; ++i) {
             cnt[i] = 0;
 #pragma unroll 1
-            for (uint32_t t = 0; t < seq[i].tiles; ++t) cnt[i] += (slabs_of<R, SLAB>(seq[i], t, group) + unit - 1) / unit;
+            for (uint32_t t = 0; t < seq[i].tiles; ++t) {
+                const uint32_t slabs = slabs_of<R, SLAB>(seq[i], t, group);
+                cnt[i] += (slabs + unit - 1) / unit + (EXTRA && slabs ? extra : 0u);
+            }
             cnt[i] *= c.kv_heads;
             sum += cnt[i];
             planes += seq[i].tiles;
@@ -155,6 +159,8 @@ __device__ __forceinline__ bool find_share(const HoloBlockCache& c, uint32_t gro
         unit = max((total + grid - planes - 1) / (grid - planes), (uint32_t)LEAST);
         want = blockIdx.x;
     } else {
+        extra = EXTRA;
+        total += EXTRA * planes;
         const uint32_t ctas = min(grid, (total + LEAST - 1) / LEAST);
         if (blockIdx.x >= ctas) return false;
         s.each = total / ctas;
@@ -166,7 +172,7 @@ __device__ __forceinline__ bool find_share(const HoloBlockCache& c, uint32_t gro
     bool found = false;
 #pragma unroll 1
     for (;; s0 += 128) {
-        if (s.apart || c.sequences > 128) count_chunk(s0);
+        if (s.apart || EXTRA || c.sequences > 128) count_chunk(s0);
         found = want < run + all;
         if (found || s0 + 128 >= c.sequences) break;
         run += all;
@@ -194,7 +200,7 @@ __device__ __forceinline__ bool find_share(const HoloBlockCache& c, uint32_t gro
     f.at = at + f.head * a_head;
     f.slabs = slabs_of<R, SLAB>(f, 0, group);
     for (;;) {
-        const uint32_t pieces = (f.slabs + unit - 1) / unit;
+        const uint32_t pieces = (f.slabs + unit - 1) / unit + (EXTRA && f.slabs ? extra : 0u);
         if (want < f.at + pieces || f.tile + 1 >= f.tiles) break;
         f.at += pieces;
         f.slabs = slabs_of<R, SLAB>(f, ++f.tile, group);
@@ -207,6 +213,10 @@ __device__ __forceinline__ bool find_share(const HoloBlockCache& c, uint32_t gro
     } else {
         s.lo = want;
         s.hi = (blockIdx.x + 1) * s.each + min(blockIdx.x + 1, s.more_by_one);
+        if (EXTRA && f.at + f.slabs <= want) {      // the share begins behind the plane's slabs
+            next_plane<R, SLAB, EXTRA>(c, group, &f);
+            if (!f.slabs || f.at >= s.hi) return false;
+        }
     }
     return true;
 }

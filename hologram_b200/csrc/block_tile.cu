@@ -12,7 +12,7 @@
 // The tiles of all planes form one list that the CTAs share out evenly; parts of a plane are joined as for few rows (block_list.cuh).
 // TMEM: S of even tiles at 0, of odd ones at 128, their weights over them, O at 256.
 // Bound: the softmax (3700 cycles a tile of 128 x 128, of which 1024 are ex2) and a plane's beginning (12 k cycles: queries, scales, first codes);
-// the workers keep up. 134 us for bf16 portions of 128, 256, 77 and 128 rows behind 2048 to 8100 positions, 32 heads over 8 of dim 128.
+// the workers keep up. 111 us for bf16 portions of 128, 256, 77 and 128 rows behind 2048 to 8100 positions, 32 heads over 8 of dim 128.
 #include "attention_issue.cuh"
 #include "block_list.cuh"
 
@@ -21,6 +21,7 @@ namespace {
 constexpr int BT_ROWS = 128, BT_TILE = 128, BT_WARPS = 16, BT_WORKERS = 128;      // threads that turn the codes of keys, and of values
 // registers a thread: the workers' and the issuer's leave what the softmax's 128 scores take (their sum is the launch's at most)
 constexpr int BT_ISSUER_REGS = 80, BT_SOFTMAX_REGS = 208, BT_WORKER_REGS = 112;
+constexpr int BT_PLANE = 3;      // tiles that a plane's beginning and end cost as much as (portions as above: 134 us where they do not count)
 constexpr float BT_GROWTH = 8.0f;
 constexpr int BT_LIFT = 7;
 
@@ -74,7 +75,7 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
     holo_pdl_wait();
     if (blockIdx.x == 0) check_sequences(c.starts, c.lengths, c.sequences, c.rows, (int64_t)c.table_ld * br, c.status);
     Share mine;
-    if (!find_share<BT_ROWS, BT_TILE, 4, 4>(c, group, &mine)) return;       // the same for every thread
+    if (!find_share<BT_ROWS, BT_TILE, 4, 4, BT_PLANE>(c, group, &mine)) return;       // the same for every thread
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -88,8 +89,8 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
     auto keys_of = [&](const Plane& f) { return (uint32_t)f.length - (f.n - rows_before<BT_ROWS>(f, f.tile, group)); };
     auto more = [&](Plane& f) {
         if (f.at + f.slabs >= mine.hi) return false;
-        next_plane<BT_ROWS, BT_TILE>(c, group, &f);
-        return f.slabs != 0;
+        next_plane<BT_ROWS, BT_TILE, BT_PLANE>(c, group, &f);
+        return f.slabs != 0 && f.at < mine.hi;
     };
 
     auto arrive_at = [&](uint32_t bar) {
@@ -560,6 +561,11 @@ int32_t launch_block_tile(holo_b200_ctx* ctx, const BlockTileParams& p) {
     static thread_local int configured_device = -1;
     if (configured_device != ctx->device) {
         HOLO_CUDA(cudaFuncSetAttribute(block_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ctx->smem_optin));
+        // the roles' registers come out of the launch's: a sum above them would be waited for without end
+        cudaFuncAttributes built;
+        HOLO_CUDA(cudaFuncGetAttributes(&built, block_tile_kernel));
+        if (built.numRegs * BT_WARPS * 32 < 128 * (BT_ISSUER_REGS + BT_SOFTMAX_REGS + 2 * BT_WORKER_REGS))
+            return holo_fail(HOLO_ERR_DISPATCH, "dispatch failed: block_cache_attention was built with %d registers a thread, too few to share out", built.numRegs);
         configured_device = ctx->device;
     }
     HOLO_CUDA(holo_launch_kernel(ctx, block_tile_kernel, dim3((uint32_t)ctx->sm_count), dim3(BT_WARPS * 32), smem, 1, p));
@@ -580,7 +586,7 @@ int32_t holo_try_block_tile(holo_b200_ctx* ctx, const HoloBlockAttnArgs& a, bool
     if ((uint64_t)c.rows * group <= 16ull * c.sequences) return HOLO_OK;
     // tiles of the whole list of 32 bits
     const uint64_t tiles = ((uint64_t)c.rows * group / BT_ROWS + c.sequences) * c.kv_heads;
-    if ((uint64_t)c.rows * a.heads > 0x7fffffffull || tiles > 0x7fffffffull / (((uint64_t)c.table_ld * c.block_rows + BT_TILE - 1) / BT_TILE)) return HOLO_OK;
+    if ((uint64_t)c.rows * a.heads > 0x7fffffffull || tiles > 0x7fffffffull / (((uint64_t)c.table_ld * c.block_rows + BT_TILE - 1) / BT_TILE + BT_PLANE)) return HOLO_OK;
     if ((uint64_t)c.blocks * c.kv_heads * c.block_rows >= 0xffffffffull) return HOLO_OK;      // row numbers of 32 bits
     HOLO_TRY(holo_block_row_partials(ctx));
     *taken = true;

@@ -498,6 +498,70 @@ def test_block_cache_reports_bad_tables(backend, what):
         backend.synchronize()
 
 
+@pytest.mark.parametrize("dtype,block", [("bf16", 16), ("f16", 24), ("f32", 16)])
+@pytest.mark.parametrize("what", ["block", "negative", "length", "short", "starts"])
+def test_block_cache_reports_bad_tables_of_portions(backend, what, dtype, block):
+    """As above where a sequence has many rows; what is not wrong is as it would be without the mistake."""
+    rng = np.random.default_rng(16)
+    cache = Cache(rng, [300, 280, 310], block, 2, 64, 64)
+    starts = [0, 70, 110, 200]
+    q = strided(rng, 200, 256, 256, dtype)
+    out = torch.zeros(200, 256, dtype=TORCH[dtype], device="cuda")
+    qf, want = f64(q).reshape(200, 4, 64), {}
+    for s, n in ((0, 300), (2, 310)):
+        a, b = starts[s], starts[s + 1]
+        k, v = cache.held("k", s, n), cache.held("v", s, n)
+        for h in range(4):
+            want[s, h] = attend(qf[a:b, h], k[:, h // 2], v[:, h // 2], n - (b - a) + 1 + np.arange(b - a), 0.125, dtype, CACHE_WEIGHT_HALF[dtype])
+    if what == "block":
+        cache.table[1, 7] = cache.blocks
+    elif what == "negative":
+        cache.table[1, 0] = -7
+    elif what == "length":
+        cache.lens[1] = cache.width * block + 1
+    elif what == "short":
+        cache.lens[1] = 12
+    else:
+        starts = [0, 70, 60, 200]
+    attention(backend, cache, q, starts, out, 4, dtype)
+    with pytest.raises(hb.BackendError, match="out of range"):
+        backend.synchronize()
+    backend.synchronize()
+    got = f64(out).reshape(200, 4, 64)
+    for h in range(4):
+        check(got[:60, h], want[0, h][0][:60], want[0, h][1][:60], "sequence 0")      # the 60 rows that are nobody else's
+        if what != "starts":
+            check(got[110:, h], *want[2, h], "sequence 2")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_portions_with_queries_of_any_size(backend, dtype):
+    """Among the rows of a portion: zeros, tiny and huge ones, one value that stands out, one that is not finite; the others take no notice."""
+    rng = np.random.default_rng(17)
+    cache = Cache(rng, [200, 90], 16, 1, 64, 64)
+    q = strided(rng, 130, 128, 128, dtype)
+    q[0] *= 1e-4
+    q[1] *= 200.0
+    q[2] = 0
+    q[3, 5] *= 1000.0
+    q[4, :64] *= 1e-3
+    q[70, 7] = float("nan")
+    q[101, 70] = float("-inf")
+    out, starts = torch.zeros(130, 128, dtype=TORCH[dtype], device="cuda"), [0, 80, 130]
+    attention(backend, cache, q, starts, out, 2, dtype)
+    backend.synchronize()
+    got, qf = f64(out).reshape(130, 2, 64), f64(q).reshape(130, 2, 64)
+    for s, n in enumerate(cache.lens):
+        k, v = cache.held("k", s, n)[:, 0], cache.held("v", s, n)[:, 0]
+        for i in range(starts[s], starts[s + 1]):
+            for h in range(2):
+                if not np.isfinite(qf[i, h]).all():
+                    assert not np.isfinite(got[i, h]).any()
+                    continue
+                want, off = attend(qf[i:i + 1, h], k, v, [n - (starts[s + 1] - 1 - i)], 0.125, dtype, CACHE_WEIGHT_HALF[dtype])
+                check(got[i:i + 1, h], want, off, f"row {i} head {h}")
+
+
 # ---- logit rules -------------------------------------------------------------------------------------------------------
 
 
