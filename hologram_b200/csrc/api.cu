@@ -1120,9 +1120,11 @@ int32_t do_causal_attention(holo_b200_ctx* ctx, const HoloCausalAttentionCall& c
 }
 
 // ---- further operations of decoder steps (all extensions) ----
+constexpr uint64_t MOST_ELEMENTS = 1ull << 50;      // of an operand: sizes in bytes stay far from 2^64
 // Resolve `rows` rows of `width` elements of pitch `ld`.
 int32_t resolve_rows(holo_b200_workspace* ws, const HoloBufferRef& ref, uint64_t rows, uint64_t ld, uint64_t width, uint64_t es, uint8_t** ptr, Range* range) {
     if (width > ld) return holo_fail(HOLO_ERR_SHAPE_MISMATCH, "shape mismatch: rows of %llu columns at a pitch of %llu", (unsigned long long)width, (unsigned long long)ld);
+    if (ld != 0 && rows > MOST_ELEMENTS / ld) return holo_fail_slot(ref.slot, "operand larger than any buffer");
     const uint64_t bytes = ((rows - 1) * ld + width) * es;
     HOLO_TRY(holo_resolve(ws, ref, bytes, ptr, nullptr));
     if (((uintptr_t)*ptr & (es - 1)) != 0) return holo_fail_slot(ref.slot, "operand must be aligned to its element on the device");
@@ -1130,6 +1132,7 @@ int32_t resolve_rows(holo_b200_workspace* ws, const HoloBufferRef& ref, uint64_t
     return HOLO_OK;
 }
 int32_t resolve_words(holo_b200_workspace* ws, const HoloBufferRef& ref, uint64_t words, uint8_t** ptr) {
+    if (words > MOST_ELEMENTS) return holo_fail_slot(ref.slot, "operand larger than any buffer");
     HOLO_TRY(holo_resolve(ws, ref, 4 * words, ptr, nullptr));
     return ((uintptr_t)*ptr & 3u) != 0 ? holo_fail_slot(ref.slot, "operand must be 4-byte aligned on the device") : HOLO_OK;
 }
@@ -1358,7 +1361,7 @@ int32_t do_packed_attention(holo_b200_ctx* ctx, const HoloPackedAttentionCall& c
 template <typename Call>
 int32_t resolve_block_cache(holo_b200_ctx* ctx, holo_b200_workspace* ws, const char* what, const Call& c, HoloBlockCache* out, Range (&r)[7]) {
     if (c.kv_heads == 0 || c.dim == 0 || c.vdim == 0 || c.dim > 512 || c.vdim > 512 || c.block_rows == 0 || c.block_rows > 1024 || c.table_ld == 0 || c.blocks == 0 ||
-        c.blocks > 0x7fffffffu || c.rows > 0x7fffffffu || c.sequences > 0x7ffffffeu || (uint64_t)c.table_ld * c.block_rows > 0x7fffffffull)
+        c.blocks > 0x7fffffffu || (uint64_t)c.blocks * c.kv_heads > MOST_ELEMENTS >> 20 || c.rows > 0x7fffffffu || c.sequences > 0x7ffffffeu || (uint64_t)c.table_ld * c.block_rows > 0x7fffffffull)
         return holo_fail(HOLO_ERR_SHAPE_MISMATCH, "shape mismatch: %s dim %u, vdim %u, %u blocks of %u rows, %u a sequence", what, c.dim, c.vdim, c.blocks, c.block_rows, c.table_ld);
     const bool singles = c.starts.slot == HOLO_NO_SLOT;
     if (singles && c.rows != c.sequences)

@@ -764,6 +764,29 @@ def test_refusals_of_logit_rules(backend):
     refused(backend, *call(change={"dtype": kc.DTYPE_I32}), "UnsupportedOp")
 
 
+def test_sizes_whose_bytes_pass_64_bits_are_refused(backend):
+    """Products of sizes that come out small modulo 2^64 are as far outside the buffers as they look."""
+    rng = np.random.default_rng(1)
+    cache, s = Cache(rng, [20], 16, 1, 64, 64), Slots(backend, 30)
+    small = lambda *shape: torch.zeros(*shape, dtype=torch.bfloat16, device="cuda")
+    refs, k, v, q, o = cache.refs(s, None), s(small(1, 64)), s(small(1, 64)), s(small(1, 64)), s(small(1, 64))
+    # 2^31 blocks of 1024 rows for 2^20 heads of 512 columns: 2^70 bytes
+    sizes = dict(rows=1, sequences=1, kv_heads=2 ** 20, dim=512, vdim=512, k_ld=2 ** 29, v_ld=2 ** 29, block_rows=1024, blocks=2 ** 31 - 1, table_ld=2, dtype=kc.DTYPE_BF16)
+    refused(backend, s, kc.KernelCall.BlockCacheWrite(kc.BlockCacheWriteCall(k, v, *refs, *sizes.values())), "ShapeMismatch")
+    sizes = dict(rows=1, sequences=1, heads=2 ** 20, kv_heads=2 ** 20, dim=512, vdim=512, q_ld=2 ** 29, ld=2 ** 29, block_rows=1024, blocks=2 ** 31 - 1, table_ld=2, scale_bits=0, dtype=kc.DTYPE_BF16)
+    refused(backend, s, kc.KernelCall.BlockCacheAttention(kc.BlockCacheAttentionCall(q, *refs, o, *sizes.values())), "ShapeMismatch")
+    z, n = s(torch.zeros(64, device="cuda")), s(torch.zeros(64, dtype=torch.int32, device="cuda"))
+    out = s(torch.zeros(64, device="cuda"))
+    # masks of 2^62 words; a history of 2^62 tokens; logits of 2^62 + 2^31 tokens less 2^31
+    for change, of in (({"mask_rows": 2 ** 31, "mask_ld": 2 ** 31}, "masks"), ({"rows": 2 ** 31 - 1, "history_ld": 2 ** 31 - 1, "ld": 1, "out_ld": 1, "vocab": 1}, "history"),
+                       ({"rows": 2 ** 30 + 1, "ld": 2 ** 32 - 1, "out_ld": 2 ** 32 - 1, "vocab": 2 ** 30}, "logits")):
+        call = dict(rows=1, vocab=64, ld=64, out_ld=64, history_ld=4, biases=0, mask_rows=1, mask_ld=2, dtype=kc.DTYPE_F32)
+        call.update(change)
+        ops = {"logits": z, "history": n if of == "history" else kc.NONE, "spans": n if of == "history" else kc.NONE, "params": z if of == "history" else kc.NONE, "bias_starts": kc.NONE,
+               "bias_ids": kc.NONE, "bias_values": kc.NONE, "masks": n if of == "masks" else kc.NONE, "mask_of": n if of == "masks" else kc.NONE, "output": out}
+        refused(backend, s, kc.KernelCall.LogitRules(kc.LogitRulesCall(*ops.values(), *call.values())), "SlotOutOfRange")
+
+
 def test_no_host_workspace_form(backend):
     host = hb.HostWorkspace([np.zeros(4096, dtype=np.uint8) for _ in range(10)])
     for call in (kc.KernelCall.PackedAttention(kc.PackedAttentionCall()), kc.KernelCall.BlockCacheWrite(kc.BlockCacheWriteCall()),
