@@ -653,11 +653,24 @@ def test_logit_rules_of_more_rows_than_a_grid_is_high(backend):
     z = strided(rng, 70000, 33, 33, "f32")
     out = torch.zeros(70000, 33, device="cuda")
     history = torch.from_numpy(rng.integers(0, 33, (70000, 3)).astype(np.int32)).cuda()
-    apply_rules(backend, z, out, history, i32([[0, 3]]).repeat(70000, 1), torch.tensor([[1.0, 0.5, 0.0, 0.0]], device="cuda").repeat(70000, 1))
+    masks = torch.full((70000, 2), -1, dtype=torch.int32, device="cuda")
+    masks[:, 1] = torch.arange(70000, device="cuda") & 1                      # odd rows may choose token 32
+    bias = i32(np.minimum(np.arange(70001), 69999).tolist()), torch.zeros(69999, dtype=torch.int32, device="cuda"), torch.arange(69999, dtype=torch.float32, device="cuda")
+    apply_rules(backend, z, out, history, i32([[0, 3]]).repeat(70000, 1), torch.tensor([[1.0, 0.5, 0.0, 0.0]], device="cuda").repeat(70000, 1), bias, masks)
     backend.synchronize()
     want = f64(z)
+    forbidden = np.arange(70000) % 2 == 0
+    assert np.all(np.isneginf(f64(out)[forbidden, 32])) and np.isfinite(f64(out)[~forbidden, 32]).all()
+    # row r has r added to its token 0, the last row nothing: another rounding of numbers up to r
+    first, more = f64(out)[:, 0], np.where(np.arange(70000) < 69999, np.arange(70000), 0)
+    seen = (history.cpu().numpy() == 0).any(1)
+    assert np.all(np.abs(first - (want[:, 0] - 0.5 * seen + more)) <= 2.0 ** -24 * (2 * np.abs(want[:, 0]) + 1 + 2 * more))
+    out[:, 0], out[:, 32], z[:, 0], z[:, 32] = 0, 0, 0, 0
+    want, history = f64(z), history.clone()
+    history[(history == 0) | (history == 32)] = -1
     seen = np.zeros((70000, 33), dtype=bool)
-    np.put_along_axis(seen, history.cpu().numpy(), True, 1)
+    for column in history.cpu().numpy().T:
+        seen[np.arange(70000)[column >= 0], column[column >= 0]] = True
     # a difference with 0.5 in f32: one rounding of a value
     assert np.all(np.abs(f64(out) - (want - 0.5 * seen)) <= 2.0 ** -24 * (np.abs(want) + 0.5))
 
