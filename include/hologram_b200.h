@@ -597,8 +597,9 @@ typedef struct HoloPackedAttentionCall {
  *   scale' = max(scale, m / 127)   (m / 127 where the block's first position is new),
  *   code = the integer nearest to x / scale' (ties to even) within [-127, 127]; infinities are +-127, NaN is 0; all 0 for scale' = 0,
  * and where a scale grows the codes of the block's earlier positions become the integers nearest to code * scale / scale'. Rows of a
- * block behind the last position, and blocks not touched, are left as they were. A block that two sequences of one call write is the
- * caller's mistake: it ends with codes and a scale of either (blocks that sequences share are full, and not written). */
+ * block behind the last position, and blocks not touched, are left as they were. A block that one call writes twice, for two sequences
+ * or in two places of one, is the caller's mistake: it ends with codes and a scale of either (blocks that sequences share are full, and
+ * not written). */
 typedef struct HoloBlockCacheWriteCall {
     HoloBufferRef k, v, starts, lengths, table, k_codes, k_scales, v_codes, v_scales;
     uint32_t rows, sequences, kv_heads, dim, vdim, k_ld, v_ld, block_rows, blocks, table_ld;
