@@ -21,7 +21,7 @@ namespace {
 constexpr int BT_ROWS = 128, BT_TILE = 128, BT_WARPS = 16, BT_WORKERS = 128;      // threads that turn the codes of keys, and of values
 // registers a thread: the workers' and the issuer's leave what the softmax's 128 scores take (their sum is the launch's at most)
 constexpr int BT_ISSUER_REGS = 80, BT_SOFTMAX_REGS = 208, BT_WORKER_REGS = 112;
-constexpr int BT_PLANE = 3;      // tiles that a plane's beginning and end cost as much as (portions as above: 134 us where they do not count)
+constexpr int BT_PLANE = 3;      // tiles that a plane's beginning and end cost as much as (portions as above, for 0, 2, 3, 4, 6: 134, 118, 110, 110, 113 us)
 constexpr float BT_GROWTH = 8.0f;
 constexpr int BT_LIFT = 7;
 
