@@ -184,7 +184,9 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const uint32_t tmem_base = *s_tmem;
     const int32_t* starts = kept ? s_starts : a.starts;
 
-    if (p.pairs <= PT_SORTED) {
+    // (the order does not matter where every item has a CTA of its own)
+    const bool sorted = p.pairs <= PT_SORTED && p.items > gridDim.x;
+    if (sorted) {
         uint32_t mine = 0;
         if (threadIdx.x < p.pairs) {
             for (uint32_t q = 0; q < p.nq; ++q) {
@@ -207,7 +209,7 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     auto make_item = [&](uint32_t i) {
         PackedItem it;
         it.head = i % a.heads;
-        it.row0 = (p.pairs <= PT_SORTED ? s_order[i / a.heads] : p.pairs - 1 - i / a.heads) * p.nq * 128;
+        it.row0 = (sorted ? s_order[i / a.heads] : p.pairs - 1 - i / a.heads) * p.nq * 128;
         KeyRange r[2];
         r[0] = keys_of_tile(a, starts, it.row0);
         r[1] = p.nq == 2 ? keys_of_tile(a, starts, it.row0 + 128) : KeyRange{0, 0};
