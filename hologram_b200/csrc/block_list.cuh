@@ -107,20 +107,20 @@ struct Share {
     }
 };
 
-// Every warp finds the share by itself, four sequences a lane at a time; false: there is none for this CTA. A share is LEAST slabs at
+// Every warp finds the share by itself, one or four sequences a lane at a time; false: there is none for this CTA. A share is LEAST slabs at
 // least, so that fewer CTAs take part in a short list. Planes are cut apart where that lengthens a share by less than the SECOND
 // slabs that another plane costs a CTA.
 template <int R, int SLAB, int LEAST, int SECOND, int EXTRA = 0>
 __device__ __forceinline__ bool find_share(const HoloBlockCache& c, uint32_t group, Share* out) {
-    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t lane = threadIdx.x & 31, each = c.sequences <= 32 ? 1u : 4u;      // of a lane
     uint32_t cnt[4], upto = 0, sum = 0, all = 0, planes = 0, unit = 1, extra = 0;
     auto count_chunk = [&](uint32_t s0) {
         Plane seq[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t s = s0 + 4 * lane + i;
+            const uint32_t s = s0 + each * lane + i;
             read_sequence<R>(c, group, min(s, c.sequences - 1), &seq[i]);
-            if (s >= c.sequences) seq[i].tiles = 0;
+            if ((uint32_t)i >= each || s >= c.sequences) seq[i].tiles = 0;
         }
         sum = 0;
 #pragma unroll
@@ -185,7 +185,7 @@ __device__ __forceinline__ bool find_share(const HoloBlockCache& c, uint32_t gro
         if (mine == 0) {
             if (want < at + cnt[i]) {
                 mine = cnt[i];
-                which = s0 + 4 * lane + i;
+                which = s0 + each * lane + i;
             } else {
                 at += cnt[i];
             }
