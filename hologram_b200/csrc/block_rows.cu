@@ -4,7 +4,7 @@
 // A CTA takes 128 query rows of a kv head (a row is a new position and a head of the group) and walks the keys in slabs of 64; two warps share
 // 16 rows, each with half of a slab's keys and a maximum, sums and a context of its own, joined at the plane's end: sixteen warps hide more
 // of each other's latency than eight with whole slabs (373 us against 472 for bf16 portions of 128, 256, 77 and 128 rows, 32 heads over 8 of
-// dim 128, behind up to 8000 positions; block_tile.cu, which has taken 16-bit rows over since, takes 111).
+// dim 128, behind up to 8000 positions; block_tile.cu, which has taken 16-bit rows over since, takes 109).
 // The codes of a slab are copied to a ring (cp.async), turned into f16 once for all warps (exact: integers of 8 bits), while the slab
 // before is worked on, and are the operands of mma.sync m16n8k16 with f32 sums. Query rows are scaled by a power of two to a largest value in
 // [2^14, 2^15), so that bf16 and f16 queries are exact in f16 (values 2^29 smaller than the largest aside); f32 queries go as two f16 terms,

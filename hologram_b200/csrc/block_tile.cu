@@ -12,7 +12,7 @@
 // The tiles of all planes form one list that the CTAs share out evenly; parts of a plane are joined as for few rows (block_list.cuh).
 // TMEM: S of even tiles at 0, of odd ones at 128, their weights over them, O at 256.
 // Bound: the softmax (3700 cycles a tile of 128 x 128, of which 1024 are ex2) and a plane's beginning (12 k cycles: queries, scales, first codes);
-// the workers keep up. 111 us for bf16 portions of 128, 256, 77 and 128 rows behind 2048 to 8100 positions, 32 heads over 8 of dim 128.
+// the workers keep up. 109 us for bf16 portions of 128, 256, 77 and 128 rows behind 2048 to 8100 positions, 32 heads over 8 of dim 128.
 #include "attention_issue.cuh"
 #include "block_list.cuh"
 
