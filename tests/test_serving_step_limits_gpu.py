@@ -1,0 +1,62 @@
+"""The calls of a serving step at their limits: scores of any size."""
+import numpy as np
+import pytest
+import torch
+
+from serving_step_reference import HALF_STEP
+from test_serving_step_gpu import CACHE_WEIGHT_HALF, TORCH, Cache, attention, check, f64, starts_of
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- scores of any size ------------------------------------------------------------------------------------------------
+
+
+def winners(codes, limits, sign, v, half, dtype):
+    """Scores are `codes` (whole numbers) times a factor that is large, its sign `sign`: a row's result is the mean of v [n, vdim] over the keys with
+    its largest score. All of those have the same score to the last bit, and the next score is lower by the factor at least: 46 and more powers
+    of two. Off by: the stored type's half step; a weight's rounding; 2^-18 for exponentials, the logarithm of a scale and the sums in f32;
+    and what the other keys' weights, 2^-46 of the largest each at most, bring in."""
+    out, off = np.zeros((len(limits), v.shape[1])), np.zeros((len(limits), v.shape[1]))
+    for i, e in enumerate(limits):
+        c = codes[:e] * sign[i]
+        top = c == c.max()
+        out[i] = v[:e][top].mean(0)
+        off[i] = 1.1 * (HALF_STEP[dtype] * np.abs(out[i]) + (half + 2.0 ** -18) * np.abs(v[:e][top]).mean(0) + e * 2.0 ** -46 * np.abs(v[:e]).max())
+    return out, off
+
+
+# the factor of the scores is 2^(power - 3) log2(e): from 46 steps a code to far beyond what f32 tells apart from its neighbours
+POWERS = [8, 12, 20, 26, 60]
+
+
+@pytest.mark.parametrize("power", POWERS)
+@pytest.mark.parametrize("dtype,block,dim,new", [
+    ("bf16", 16, 64, [70, 40]), ("f16", 32, 128, [70, 40]), ("bf16", 48, 80, [300]),       # portions on the tensor cores
+    ("bf16", 24, 64, [70, 40]), ("f32", 16, 64, [70, 40]), ("f16", 24, 128, [130]),        # portions of odd blocks, of f32
+    ("bf16", 16, 64, [1, 1]), ("f16", 24, 128, [2, 1]), ("f32", 16, 128, [1, 1]),          # few rows
+    ("bf16", 16, 40, [3, 1]),                                                              # any shape
+])
+def test_block_cache_attention_of_scores_of_any_size(backend, dtype, block, dim, new, power):
+    """Query rows with one value of 1 or -1, key scales of 1: a score is a code times the call's scale."""
+    rng = np.random.default_rng(19)
+    cache = Cache(rng, [n + 260 for n in new], block, 1, dim, dim)
+    cache.host["k_scales"][:] = 1.0
+    cache.dev["k_scales"].fill_(1.0)
+    starts, rows = starts_of(new), sum(new)
+    sign, column = rng.choice([-1.0, 1.0], (rows, 2)), rng.integers(0, dim, (rows, 2))
+    q = torch.zeros(rows, 2, dim)
+    for r in range(rows):
+        for h in range(2):
+            q[r, h, column[r, h]] = sign[r, h]
+    q, out = q.reshape(rows, 2 * dim).to(TORCH[dtype]).cuda(), torch.zeros(rows, 2 * dim, dtype=TORCH[dtype], device="cuda")
+    attention(backend, cache, q, starts, out, 2, dtype, scale=2.0 ** (power - 3))
+    backend.synchronize()
+    got = f64(out).reshape(rows, 2, dim)
+    for s, n in enumerate(cache.lens):
+        k, v = cache.held("k", s, n)[:, 0], cache.held("v", s, n)[:, 0]
+        for i in range(new[s]):
+            for h in range(2):
+                r = int(starts[s]) + i
+                want, off = winners(k[:, column[r, h]], [n - new[s] + 1 + i], [sign[r, h]], v, CACHE_WEIGHT_HALF[dtype], dtype)
+                check(got[r:r + 1, h], want, off, f"row {r} head {h}")
