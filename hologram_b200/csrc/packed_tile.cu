@@ -450,7 +450,8 @@ packed_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const float inv = __fdiv_rn(1.0f, sum);
-            const bool nothing = sum == 0.0f;       // every score -inf
+            // every score -inf (a sum of 0 under a finite maximum: exponents of far scores were off, which the row is done again for)
+            const bool nothing = sum == 0.0f && top == -INFINITY;
             uint16_t* out = (uint16_t*)a.out + (uint64_t)row * a.ld + (uint64_t)it.head * a.vdim;
             bool finite = true;
             for (uint32_t c = 0; c < a.vdim; c += 16) {

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from serving_step_reference import HALF_STEP
-from test_serving_step_gpu import CACHE_WEIGHT_HALF, TORCH, Cache, attention, check, f64, starts_of
+from test_serving_step_gpu import CACHE_WEIGHT_HALF, TORCH, WEIGHT_HALF, Cache, attention, check, f64, packed, starts_of, strided
 
 pytestmark = pytest.mark.gpu
 
@@ -59,4 +59,29 @@ def test_block_cache_attention_of_scores_of_any_size(backend, dtype, block, dim,
             for h in range(2):
                 r = int(starts[s]) + i
                 want, off = winners(k[:, column[r, h]], [n - new[s] + 1 + i], [sign[r, h]], v, CACHE_WEIGHT_HALF[dtype], dtype)
+                check(got[r:r + 1, h], want, off, f"row {r} head {h}")
+
+
+@pytest.mark.parametrize("power", POWERS)
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("f16", 128), ("bf16", 80), ("f32", 64), ("bf16", 40)])
+def test_packed_attention_of_scores_of_any_size(backend, dtype, dim, power):
+    """As over the cache: keys of whole numbers of at most 7 bits, which all types hold."""
+    rng = np.random.default_rng(20)
+    lens = [300, 40, 150]
+    starts, rows = starts_of(lens), sum(lens)
+    sign, column = rng.choice([-1.0, 1.0], (rows, 2)), rng.integers(0, dim, (rows, 2))
+    q = torch.zeros(rows, 2, dim)
+    for r in range(rows):
+        for h in range(2):
+            q[r, h, column[r, h]] = sign[r, h]
+    q = q.reshape(rows, 2 * dim).to(TORCH[dtype]).cuda()
+    k = torch.from_numpy(rng.integers(-127, 128, (rows, dim)).astype(np.float32)).to(TORCH[dtype]).cuda()
+    v, out = strided(rng, rows, dim, dim, dtype), torch.zeros(rows, 2 * dim, dtype=TORCH[dtype], device="cuda")
+    packed(backend, q, k, v, starts, out, 2, 1, dim, dim, True, dtype, scale=2.0 ** (power - 3))
+    backend.synchronize()
+    got, kf, vf = f64(out).reshape(rows, 2, dim), f64(k), f64(v)
+    for a, b in zip(starts, starts[1:]):
+        for r in range(a, b):
+            for h in range(2):
+                want, off = winners(kf[a:b, column[r, h]], [r + 1 - a], [sign[r, h]], vf[a:b], WEIGHT_HALF[dtype], dtype)
                 check(got[r:r + 1, h], want, off, f"row {r} head {h}")
