@@ -97,7 +97,7 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
     auto enter_ahead = [&]() {
         mine.ends_of(ahead, &ahead_slab, &ahead_end);
         ahead_slab += warp;
-        ahead_sees = (uint32_t)ahead.length - (ahead.n - rows_before<R>(ahead, ahead.tile, group));
+        ahead_sees = keys_of_plane<R>(ahead, ahead.tile, group);
         load_ids(block_of(ahead_slab * BA_SLAB));
     };
     auto find_ahead = [&]() {

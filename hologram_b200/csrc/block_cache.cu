@@ -293,25 +293,26 @@ struct CacheSource {
         uint32_t from = row, to = row + 1;
         p->sequence = row;
         if (a.c.starts && !sequence_of(a.c.starts, a.c.sequences, a.c.rows, row, &from, &to, &p->sequence)) return false;
-        const int64_t most = (int64_t)a.c.table_ld * a.c.block_rows, sees = (int64_t)a.c.lengths[p->sequence] - to + row + 1;
+        const int64_t most = (int64_t)a.c.table_ld * a.c.block_rows, length = max((int64_t)0, min((int64_t)a.c.lengths[p->sequence], most));
         p->begin = 0;
-        p->end = (uint32_t)max((int64_t)0, min(sees, most));
+        p->end = (uint32_t)max((int64_t)0, length - to + row + 1);
         return true;
     }
     __device__ float q(uint32_t row, uint32_t head, uint32_t x) const { return seq_load(a.q, (uint64_t)row * a.q_ld + (uint64_t)head * a.c.dim + x, a.dtype); }
-    __device__ bool key(const Place& at, uint32_t head, uint32_t j, uint64_t* kb, uint64_t* vb, float* ks, float* vs) const {
+    __device__ void key(const Place& at, uint32_t head, uint32_t j, uint64_t* kb, uint64_t* vb, float* ks, float* vs) const {
         const uint32_t br = a.c.block_rows;
         const int id = a.c.table[(uint64_t)at.sequence * a.c.table_ld + j / br];
-        if (id < 0 || (uint32_t)id >= a.c.blocks) {
+        if (id < 0 || (uint32_t)id >= a.c.blocks) {      // a block of zeros
             atomicOr(a.c.status, HOLO_STATUS_TABLE);
-            return false;
+            *kb = *vb = 0;
+            *ks = *vs = 0.0f;
+            return;
         }
         const uint64_t plane = (uint64_t)id * a.c.kv_heads + head / (a.heads / a.c.kv_heads), row = plane * br + j % br;
         *kb = row * a.c.dim;
         *vb = row * a.c.vdim;
         *ks = a.c.k_scales[plane];
         *vs = a.c.v_scales[plane];
-        return true;
     }
     __device__ float k(uint64_t i) const { return (float)a.c.k_codes[i]; }
     __device__ float v(uint64_t i) const { return (float)a.c.v_codes[i]; }

@@ -44,10 +44,15 @@ template <int R>
 __device__ __forceinline__ uint32_t rows_before(const Plane& p, uint32_t tile, uint32_t group) {       // positions up to the tile's last one
     return min(p.n, (tile * R + R - 1) / group + 1);
 }
+// Positions that the tile's last row sees. None happens to sequences with fewer positions than rows (reported by check_sequences): their planes
+// have a slab all the same, whose keys are beyond every row's limit, so that rows that see nothing are stored as zeros.
+template <int R>
+__device__ __forceinline__ uint32_t keys_of_plane(const Plane& p, uint32_t tile, uint32_t group) {
+    return (uint32_t)max(1, p.length - (int32_t)(p.n - rows_before<R>(p, tile, group)));
+}
 template <int R, int SLAB>
 __device__ __forceinline__ uint32_t slabs_of(const Plane& p, uint32_t tile, uint32_t group) {
-    const int32_t sees = p.length - (int32_t)(p.n - rows_before<R>(p, tile, group));
-    return sees <= 0 ? 0u : ((uint32_t)sees + SLAB - 1) / SLAB;
+    return (keys_of_plane<R>(p, tile, group) + SLAB - 1) / SLAB;
 }
 template <int R>
 __device__ __forceinline__ void read_sequence(const HoloBlockCache& c, uint32_t group, uint32_t s, Plane* p) {
@@ -64,7 +69,7 @@ __device__ __forceinline__ void read_sequence(const HoloBlockCache& c, uint32_t 
     p->tiles = (p->n * group + R - 1) / R;
     p->head = p->tile = 0;
 }
-// On to the next plane that has slabs; slabs == 0: there is none. EXTRA: places of the list behind a plane's slabs that stand for what a
+// On to the next plane; slabs == 0: there is none. EXTRA: places of the list behind a plane's slabs that stand for what a
 // plane costs a CTA beside them.
 template <int R, int SLAB, int EXTRA = 0>
 __device__ __forceinline__ void next_plane(const HoloBlockCache& c, uint32_t group, Plane* p) {
@@ -80,9 +85,11 @@ __device__ __forceinline__ void next_plane(const HoloBlockCache& c, uint32_t gro
                 read_sequence<R>(c, group, p->seq, p);
             }
         }
-        p->slabs = p->tiles ? slabs_of<R, SLAB>(*p, p->tile, group) : 0u;
-        if (p->slabs) return;
-        if (!p->tiles) p->head = c.kv_heads - 1;
+        if (p->tiles) {
+            p->slabs = slabs_of<R, SLAB>(*p, p->tile, group);
+            return;
+        }
+        p->head = c.kv_heads - 1;      // no rows: on to the next sequence
     }
 }
 
@@ -128,8 +135,7 @@ __device__ __forceinline__ bool find_share(const HoloBlockCache& c, uint32_t gro
             cnt[i] = 0;
 #pragma unroll 1
             for (uint32_t t = 0; t < seq[i].tiles; ++t) {
-                const uint32_t slabs = slabs_of<R, SLAB>(seq[i], t, group);
-                cnt[i] += (slabs + unit - 1) / unit + (EXTRA && slabs ? extra : 0u);
+                cnt[i] += (slabs_of<R, SLAB>(seq[i], t, group) + unit - 1) / unit + (EXTRA ? extra : 0u);
             }
             cnt[i] *= c.kv_heads;
             sum += cnt[i];
@@ -200,7 +206,7 @@ __device__ __forceinline__ bool find_share(const HoloBlockCache& c, uint32_t gro
     f.at = at + f.head * a_head;
     f.slabs = slabs_of<R, SLAB>(f, 0, group);
     for (;;) {
-        const uint32_t pieces = (f.slabs + unit - 1) / unit + (EXTRA && f.slabs ? extra : 0u);
+        const uint32_t pieces = (f.slabs + unit - 1) / unit + (EXTRA ? extra : 0u);
         if (want < f.at + pieces || f.tile + 1 >= f.tiles) break;
         f.at += pieces;
         f.slabs = slabs_of<R, SLAB>(f, ++f.tile, group);

@@ -65,7 +65,7 @@ block_rows_kernel(const __grid_constant__ BlockRowsParams p) {
     for (;;) {
         uint32_t s0, s1;
         mine.ends_of(at, &s0, &s1);
-        const uint32_t rows = min((uint32_t)BR_ROWS, at.n * group - at.tile * BR_ROWS), sees = (uint32_t)at.length - (at.n - rows_before<BR_ROWS>(at, at.tile, group));
+        const uint32_t rows = min((uint32_t)BR_ROWS, at.n * group - at.tile * BR_ROWS), sees = keys_of_plane<BR_ROWS>(at, at.tile, group);
         // block numbers of a slab's keys, a slab ahead of the copies
         int id_k[UNITS], id_v[UNITS], id_s = -1;
         auto find = [&](uint32_t slab, int key) {

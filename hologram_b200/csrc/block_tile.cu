@@ -90,7 +90,7 @@ block_tile_kernel(const __grid_constant__ BlockTileParams p) {
     holo_pdl_trigger();
     const uint32_t tmem_base = *s_tmem;
     // everybody walks the planes by itself
-    auto keys_of = [&](const Plane& f) { return (uint32_t)f.length - (f.n - rows_before<BT_ROWS>(f, f.tile, group)); };
+    auto keys_of = [&](const Plane& f) { return keys_of_plane<BT_ROWS>(f, f.tile, group); };
     auto more = [&](Plane& f) {
         if (f.at + f.slabs >= mine.hi) return false;
         next_plane<BT_ROWS, BT_TILE, BT_PLANE>(c, group, &f);

@@ -21,12 +21,11 @@ struct PackedSource {
         return true;
     }
     __device__ float q(uint32_t row, uint32_t head, uint32_t c) const { return seq_load(a.q, (uint64_t)row * a.q_ld + (uint64_t)head * a.dim + c, a.dtype); }
-    __device__ bool key(const Place&, uint32_t head, uint32_t j, uint64_t* kb, uint64_t* vb, float* ks, float* vs) const {
+    __device__ void key(const Place&, uint32_t head, uint32_t j, uint64_t* kb, uint64_t* vb, float* ks, float* vs) const {
         const uint32_t g = head / (a.heads / a.kv_heads);
         *kb = (uint64_t)j * a.k_ld + (uint64_t)g * a.dim;
         *vb = (uint64_t)j * a.v_ld + (uint64_t)g * a.vdim;
         *ks = *vs = 1.0f;
-        return true;
     }
     __device__ float k(uint64_t i) const { return seq_load(a.k, i, a.dtype); }
     __device__ float v(uint64_t i) const { return seq_load(a.v, i, a.dtype); }

@@ -83,7 +83,7 @@ general_rows_kernel(const __grid_constant__ Source src) {
         for (uint32_t j = at.begin + warp; j < at.end; j += SEQ_WARPS) {
             uint64_t kb, vb;
             float ks, vs;
-            if (!src.key(at, head, j, &kb, &vb, &ks, &vs)) continue;
+            src.key(at, head, j, &kb, &vb, &ks, &vs);
             float s = 0.0f;
 #pragma unroll
             for (int i = 0; i < SEQ_PER_LANE; ++i) {

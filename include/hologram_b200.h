@@ -590,7 +590,9 @@ typedef struct HoloPackedAttentionCall {
  * included. The call's rows are packed: sequence s has rows [starts[s], starts[s + 1]), which are its last positions (starts absent:
  * row s is the one row of sequence s, and `rows` is `sequences`). Entries of the table behind a sequence's positions are not read.
  * A block number outside [0, blocks), starts that descend or leave [0, rows] and lengths below a sequence's number of rows or above
- * table_ld * block_rows are reported at the next synchronising call; nothing is read or written outside the buffers for them. */
+ * table_ld * block_rows are reported at the next synchronising call; nothing is read or written outside the buffers for them. Writing
+ * leaves out such blocks and sequences. Attention takes a length below 0 for 0 and one above for the table's positions, and a block that does not
+ * exist for one of zeros; what becomes of the rows of sequences whose starts are out of range is not defined. */
 
 /* Extension. k [rows, kv_heads * dim] (pitch k_ld) and v [rows, kv_heads * vdim] (pitch v_ld), `dtype` f32, bf16 or f16, into the
  * cache, after which lengths hold. For each block and head touched, m the largest finite magnitude of its new rows:

@@ -1,9 +1,10 @@
-"""The calls of a serving step at their limits: scores of any size."""
+"""The calls of a serving step at their limits: scores of any size, lengths and block numbers out of range."""
 import numpy as np
 import pytest
 import torch
 
-from serving_step_reference import HALF_STEP
+import hologram_b200 as hb
+from serving_step_reference import HALF_STEP, attend
 from test_serving_step_gpu import CACHE_WEIGHT_HALF, TORCH, WEIGHT_HALF, Cache, attention, check, f64, packed, starts_of, strided
 
 pytestmark = pytest.mark.gpu
@@ -85,3 +86,46 @@ def test_packed_attention_of_scores_of_any_size(backend, dtype, dim, power):
             for h in range(2):
                 want, off = winners(kf[a:b, column[r, h]], [r + 1 - a], [sign[r, h]], vf[a:b], WEIGHT_HALF[dtype], dtype)
                 check(got[r:r + 1, h], want, off, f"row {r} head {h}")
+
+
+# ---- lengths and block numbers out of range ----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("what", ["nothing", "negative", "short", "long", "block", "no block"])
+@pytest.mark.parametrize("dtype,block,dim,new", [
+    ("bf16", 16, 64, [40, 37, 50]), ("f16", 24, 64, [40, 37, 50]), ("f32", 16, 64, [40, 37, 50]),      # portions: tensor cores, odd blocks, f32
+    ("bf16", 32, 64, [1, 1, 1]), ("f32", 16, 128, [2, 3, 1]), ("f16", 24, 64, [1, 3, 2]),              # few rows
+    ("bf16", 16, 40, [2, 3, 1]), ("f32", 8, 33, [20, 30, 10]),                                         # any shape
+])
+def test_what_is_out_of_range_counts_the_same_in_every_shape(backend, what, dtype, block, dim, new):
+    """Reported, and: a length counts as 0 below and as the table's positions above, rows that see nothing are zero, a block that does not
+    exist holds zeros."""
+    rng = np.random.default_rng(21)
+    cache = Cache(rng, [90, 110, 130], block, 2, dim, dim)
+    starts, rows = starts_of(new), sum(new)
+    q, out = strided(rng, rows, 4 * dim, 4 * dim, dtype), torch.full((rows, 4 * dim), 5.0, dtype=TORCH[dtype], device="cuda")
+    k, v = [[cache.held(p, s, n) for s, n in enumerate(cache.lens)] for p in "kv"]
+    length = cache.lens[1]
+    if what in ("block", "no block"):
+        cache.table[1, 1] = cache.blocks if what == "block" else -1
+        for x in (k[1], v[1]):
+            x[block:2 * block] = 0
+    elif what == "long":
+        # every block of the table is one of the cache's, so that only the length is wrong
+        cache.table[cache.table < 0] = 0
+        length = cache.width * block
+        k[1], v[1] = cache.held("k", 1, length), cache.held("v", 1, length)
+        cache.lens[1] = length + 9
+    else:
+        cache.lens[1] = {"nothing": 0, "negative": -4, "short": new[1] // 2}[what]
+        length = max(cache.lens[1], 0)
+    attention(backend, cache, q, starts, out, 4, dtype)
+    with pytest.raises(hb.BackendError, match="out of range"):
+        backend.synchronize()
+    backend.synchronize()
+    got, qf = f64(out).reshape(rows, 4, dim), f64(q).reshape(rows, 4, dim)
+    for s, n in enumerate([cache.lens[0], length, cache.lens[2]]):
+        a, b = int(starts[s]), int(starts[s + 1])
+        for h in range(4):
+            want, off = attend(qf[a:b, h], k[s][:, h // 2], v[s][:, h // 2], n - (b - a) + 1 + np.arange(b - a), dim ** -0.5, dtype, CACHE_WEIGHT_HALF[dtype])
+            check(got[a:b, h], want, off, f"sequence {s}")
