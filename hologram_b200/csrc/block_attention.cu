@@ -478,26 +478,34 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
 
 constexpr uint32_t BA_MOST_CTAS = 3 * 192;
 
+// 16-byte units of 8 neighbouring rows on different banks: an odd number of them a row, or units moved by the row's number
+constexpr uint32_t ba_pitch(uint32_t d) { return d % 128 == 0 || (d / 16) % 2 == 1 ? d : d + 16; }
+constexpr uint32_t ba_slab_bytes(uint32_t k_pitch, uint32_t v_pitch) { return BA_SLAB * (k_pitch + v_pitch) + 256; }
+// the digits; then the warps' results; then the weights of a plane's parts
+constexpr uint32_t ba_head_bytes(uint32_t rt, uint32_t maxd, uint32_t vdim, uint32_t ctas) {
+    const uint32_t digits = rt * 16 * maxd, merge = BA_WARPS * 4 * rt * vdim * 4, weights = 16 * rt * ctas, most = digits > merge ? digits : merge;
+    return ((most > weights ? most : weights) + 127u) & ~127u;
+}
+// what no call of an instance goes beyond
+constexpr uint32_t ba_most_bytes(uint32_t rt, uint32_t maxd, uint32_t stages) {
+    uint32_t pitch = 0;
+    for (uint32_t d = 16; d <= maxd; d += 16) pitch = ba_pitch(d) > pitch ? ba_pitch(d) : pitch;
+    return ba_head_bytes(rt, maxd, maxd, BA_MOST_CTAS) + BA_WARPS * stages * ba_slab_bytes(pitch, pitch);
+}
+
 template <int RT, int MAXD, bool EXACT, bool SECOND, int STAGES, int CTAS>
 int32_t launch_block_attention(holo_b200_ctx* ctx, BlockAttnParams& p) {
-    const uint32_t dim = p.a.c.dim, vdim = p.a.c.vdim;
-    // 16-byte units of 8 neighbouring rows on different banks: an odd number of them a row, or units moved by the row's number
-    auto pitch = [](uint32_t d) { return d % 128 == 0 || (d / 16) % 2 == 1 ? d : d + 16; };
-    p.k_pitch = pitch(dim);
-    p.v_pitch = pitch(vdim);
-    p.slab_bytes = BA_SLAB * (p.k_pitch + p.v_pitch) + 256;
-    const uint32_t digits = RT * 16 * MAXD, merge = BA_WARPS * 4 * RT * vdim * 4;
     const uint32_t ctas = (uint32_t)ctx->sm_count * CTAS < BA_MOST_CTAS ? (uint32_t)ctx->sm_count * CTAS : BA_MOST_CTAS;
-    p.head_bytes = digits > merge ? digits : merge;
-    if (p.head_bytes < 16 * RT * ctas) p.head_bytes = 16 * RT * ctas;      // the weights of a plane's parts
-    p.head_bytes = (p.head_bytes + 127u) & ~127u;
+    p.k_pitch = ba_pitch(p.a.c.dim);
+    p.v_pitch = ba_pitch(p.a.c.vdim);
+    p.slab_bytes = ba_slab_bytes(p.k_pitch, p.v_pitch);
+    p.head_bytes = ba_head_bytes(RT, MAXD, p.a.c.vdim, ctas);
     const uint32_t smem = p.head_bytes + BA_WARPS * STAGES * p.slab_bytes;
     static thread_local int configured_device = -1;
-    static thread_local uint32_t configured = 0;
-    if (configured_device != ctx->device || configured < smem) {
-        HOLO_CUDA(cudaFuncSetAttribute(block_attention_kernel<RT, MAXD, EXACT, SECOND, STAGES, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (configured_device != ctx->device) {
+        // the attribute is the process's: every thread sets the same, whatever sizes its calls have
+        HOLO_CUDA(cudaFuncSetAttribute(block_attention_kernel<RT, MAXD, EXACT, SECOND, STAGES, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ba_most_bytes(RT, MAXD, STAGES)));
         configured_device = ctx->device;
-        configured = smem;
     }
     HOLO_CUDA(holo_launch_kernel(ctx, block_attention_kernel<RT, MAXD, EXACT, SECOND, STAGES, CTAS>, dim3(ctas), dim3(BA_THREADS), smem, 1, p));
     ctx->launches++;

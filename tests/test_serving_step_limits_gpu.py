@@ -1,4 +1,6 @@
-"""The calls of a serving step at their limits: scores of any size, lengths and block numbers out of range."""
+"""The calls of a serving step at their limits: scores of any size, lengths and block numbers out of range, threads with heads of different sizes."""
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 import torch
@@ -129,3 +131,44 @@ def test_what_is_out_of_range_counts_the_same_in_every_shape(backend, what, dtyp
         for h in range(4):
             want, off = attend(qf[a:b, h], k[s][:, h // 2], v[s][:, h // 2], n - (b - a) + 1 + np.arange(b - a), dim ** -0.5, dtype, CACHE_WEIGHT_HALF[dtype])
             check(got[a:b, h], want, off, f"sequence {s}")
+
+
+# ---- threads -----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("large,small", [((112, 128), (80, 80)), ((48, 64), (16, 16)), ((240, 256), (144, 144))])
+@pytest.mark.parametrize("new", [[1, 1], [2, 1]])
+def test_threads_with_heads_of_different_sizes(large, small, new):
+    """Two threads, a context each, whose calls want different amounts of shared memory of one kernel: the smaller one's takes nothing from the
+    larger one's."""
+    def make(dims, seed):
+        be, rng = hb.B200Backend(0), np.random.default_rng(seed)
+        dim, vdim = dims
+        cache = Cache(rng, [300, 77], 16, 2, dim, vdim)
+        q, out = strided(rng, sum(new), 4 * dim, 4 * dim, "bf16"), torch.zeros(sum(new), 4 * vdim, dtype=torch.bfloat16, device="cuda")
+        return be, cache, q, out
+
+    def run(made):
+        be, cache, q, out = made
+        out.zero_()
+        kept = attention(be, cache, q, starts_of(new), out, 4, "bf16")
+        be.synchronize()
+        got, starts = f64(out).reshape(sum(new), 4, cache.vdim), starts_of(new)
+        for s, n in enumerate(cache.lens):
+            a, b = int(starts[s]), int(starts[s + 1])
+            k, v = cache.held("k", s, n), cache.held("v", s, n)
+            for h in range(4):
+                want, off = attend(f64(q).reshape(-1, 4, cache.dim)[a:b, h], k[:, h // 2], v[:, h // 2], n - (b - a) + 1 + np.arange(b - a), cache.dim ** -0.5, "bf16",
+                                   CACHE_WEIGHT_HALF["bf16"])
+                check(got[a:b, h], want, off, f"sequence {s}")
+        del kept
+
+    with ThreadPoolExecutor(1) as one, ThreadPoolExecutor(1) as other:
+        first, second = one.submit(make, large, 41).result(), other.submit(make, small, 42).result()
+        try:
+            for _ in range(2):
+                one.submit(run, first).result()
+                other.submit(run, second).result()
+        finally:
+            one.submit(first[0].close).result()
+            other.submit(second[0].close).result()
