@@ -38,6 +38,13 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Two CTAs an SM have some 114 KB each: the results of eight rows of 128 columns, 16 KB for four warps, are joined in two passes of 64 columns.
+// In one pass a CTA takes 118 KB, an SM holds one, and the list, cut for two, is worked through in two turns. One pass and two, dim 128: 64
+// sequences of 4096 positions, 16 heads over 2, 63.2 and 40.3 us, 8 over 1 40.9 and 27.8; two rows of each, 32 over 8, 159 and 102; eight
+// sequences of 1000, 16 over 2, 14.5 and 16.5; one of 30000 34.3 and 35.7.
+template <int RT, int MAXD, bool EXACT>
+constexpr uint32_t BA_PASSES = RT == 2 && MAXD == 128 && EXACT ? 2 : 1;
+
 // RT: four query rows or eight. D: dim and vdim where both are MAXD (their steps are constants then), else 0. SECOND: eight rows' weights
 // as two terms.
 template <int RT, int MAXD, bool EXACT, bool SECOND, int STAGES, int CTAS>
@@ -356,8 +363,9 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
             if (next.slabs) load_rows(next);
         }
         float* partial = p.partials + ((uint64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * R * (vdim + 2);
-        float* s_o = reinterpret_cast<float*>(smem);       // [warp][R][vdim]
-        const uint32_t columns = vdim / 4;
+        float* s_o = reinterpret_cast<float*>(smem);       // [warp][R][columns of a pass]
+        constexpr uint32_t PASSES = BA_PASSES<RT, MAXD, EXACT>, STEPS = CHUNKS / PASSES;
+        const uint32_t columns = vdim / 4, across = vdim / PASSES;      // units of four; columns of a pass
         auto store4 = [&](uint32_t r, uint32_t col, float4 v) {
             const uint32_t flat = at.tile * R + r;
             const uint64_t index = (uint64_t)(at.first_row + flat / group) * a.ld + (uint64_t)(at.head * group + flat % group) * vdim + col;
@@ -372,42 +380,46 @@ block_attention_kernel(const __grid_constant__ BlockAttnParams p) {
         };
         __syncthreads();        // the digits have been read
 #pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) {
-            if (!EXACT && 16 * i >= vdim) break;
-            float y[4];
+        for (uint32_t pass = 0; pass < PASSES; ++pass) {
+            if (pass) __syncthreads();      // the last pass's have been read
 #pragma unroll
-            for (int x = 0; x < 4; ++x) y[x] = RT == 1 ? o[i][x] + __shfl_xor_sync(0xffffffffu, o[i][x], 2) : o[i][x];
-            if (RT == 2 || in_quad < 2) {
-                float* to4 = s_o + (warp * R + 2 * in_quad) * vdim + 16 * i + 2 * quad;
-                *reinterpret_cast<float2*>(to4) = make_float2(y[0], y[2]);
-                *reinterpret_cast<float2*>(to4 + vdim) = make_float2(y[1], y[3]);
-            }
-        }
-        __syncthreads();
-        for (uint32_t i = tid; i < rows * columns; i += BA_THREADS) {
-            const uint32_t r = i / columns, col = 4 * (i % columns);
-            float m = -INFINITY, l = 0.0f;
+            for (uint32_t i = pass * STEPS; i < (pass + 1) * STEPS; ++i) {
+                if (!EXACT && 16 * i >= vdim) break;
+                float y[4];
 #pragma unroll
-            for (int w = 0; w < BA_WARPS; ++w) m = fmaxf(m, s_ml[w][r][0]);
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < BA_WARPS; ++w) {
-                const float lw = s_ml[w][r][1];
-                if (lw != 0.0f) {       // NaN is not 0
-                    const float f = ex2(s_ml[w][r][0] - m), g = f * s_ml[w][r][2];
-                    const float4 y = *reinterpret_cast<const float4*>(s_o + (w * R + r) * vdim + col);
-                    l = fmaf(f, lw, l);
-                    v = make_float4(fmaf(g, y.x, v.x), fmaf(g, y.y, v.y), fmaf(g, y.z, v.z), fmaf(g, y.w, v.w));
+                for (int x = 0; x < 4; ++x) y[x] = RT == 1 ? o[i][x] + __shfl_xor_sync(0xffffffffu, o[i][x], 2) : o[i][x];
+                if (RT == 2 || in_quad < 2) {
+                    float* to4 = s_o + (warp * R + 2 * in_quad) * across + 16 * (i - pass * STEPS) + 2 * quad;
+                    *reinterpret_cast<float2*>(to4) = make_float2(y[0], y[2]);
+                    *reinterpret_cast<float2*>(to4 + across) = make_float2(y[1], y[3]);
                 }
             }
-            if (whole) {
-                const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-                store4(r, col, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-            } else {
-                float* to2 = partial + r * (vdim + 2);
-                __stcg(reinterpret_cast<float2*>(to2 + col), make_float2(v.x, v.y));
-                __stcg(reinterpret_cast<float2*>(to2 + col + 2), make_float2(v.z, v.w));
-                if (col == 0) __stcg(reinterpret_cast<float2*>(to2 + vdim), make_float2(m, l));
+            __syncthreads();
+            for (uint32_t i = tid; i < rows * (across / 4); i += BA_THREADS) {
+                const uint32_t r = i / (across / 4), x = 4 * (i % (across / 4)), col = pass * across + x;
+                float m = -INFINITY, l = 0.0f;
+#pragma unroll
+                for (int w = 0; w < BA_WARPS; ++w) m = fmaxf(m, s_ml[w][r][0]);
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < BA_WARPS; ++w) {
+                    const float lw = s_ml[w][r][1];
+                    if (lw != 0.0f) {       // NaN is not 0
+                        const float f = ex2(s_ml[w][r][0] - m), g = f * s_ml[w][r][2];
+                        const float4 y = *reinterpret_cast<const float4*>(s_o + (w * R + r) * across + x);
+                        l = fmaf(f, lw, l);
+                        v = make_float4(fmaf(g, y.x, v.x), fmaf(g, y.y, v.y), fmaf(g, y.z, v.z), fmaf(g, y.w, v.w));
+                    }
+                }
+                if (whole) {
+                    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+                    store4(r, col, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                } else {
+                    float* to2 = partial + r * (vdim + 2);
+                    __stcg(reinterpret_cast<float2*>(to2 + col), make_float2(v.x, v.y));
+                    __stcg(reinterpret_cast<float2*>(to2 + col + 2), make_float2(v.z, v.w));
+                    if (col == 0) __stcg(reinterpret_cast<float2*>(to2 + vdim), make_float2(m, l));
+                }
             }
         }
         if (!whole) {
@@ -481,9 +493,9 @@ constexpr uint32_t BA_MOST_CTAS = 3 * 192;
 // 16-byte units of 8 neighbouring rows on different banks: an odd number of them a row, or units moved by the row's number
 constexpr uint32_t ba_pitch(uint32_t d) { return d % 128 == 0 || (d / 16) % 2 == 1 ? d : d + 16; }
 constexpr uint32_t ba_slab_bytes(uint32_t k_pitch, uint32_t v_pitch) { return BA_SLAB * (k_pitch + v_pitch) + 256; }
-// the digits; then the warps' results; then the weights of a plane's parts
-constexpr uint32_t ba_head_bytes(uint32_t rt, uint32_t maxd, uint32_t vdim, uint32_t ctas) {
-    const uint32_t digits = rt * 16 * maxd, merge = BA_WARPS * 4 * rt * vdim * 4, weights = 16 * rt * ctas, most = digits > merge ? digits : merge;
+// the digits; then the warps' results, `columns` of them at a time; then the weights of a plane's parts
+constexpr uint32_t ba_head_bytes(uint32_t rt, uint32_t maxd, uint32_t columns, uint32_t ctas) {
+    const uint32_t digits = rt * 16 * maxd, merge = BA_WARPS * 4 * rt * columns * 4, weights = 16 * rt * ctas, most = digits > merge ? digits : merge;
     return ((most > weights ? most : weights) + 127u) & ~127u;
 }
 // what no call of an instance goes beyond
@@ -495,11 +507,15 @@ constexpr uint32_t ba_most_bytes(uint32_t rt, uint32_t maxd, uint32_t stages) {
 
 template <int RT, int MAXD, bool EXACT, bool SECOND, int STAGES, int CTAS>
 int32_t launch_block_attention(holo_b200_ctx* ctx, BlockAttnParams& p) {
+    constexpr uint32_t PASSES = BA_PASSES<RT, MAXD, EXACT>;
+    // 228 KB an SM, of which every CTA takes 1 KB for itself and has 512 bytes of static variables; the other dims are below these
+    static_assert(!EXACT || CTAS * (ba_head_bytes(RT, MAXD, MAXD / PASSES, 148 * CTAS) + BA_WARPS * STAGES * ba_slab_bytes(ba_pitch(MAXD), ba_pitch(MAXD)) + 1536) <= 228 * 1024,
+                  "the CTAs that an SM is to hold do not fit");
     const uint32_t ctas = (uint32_t)ctx->sm_count * CTAS < BA_MOST_CTAS ? (uint32_t)ctx->sm_count * CTAS : BA_MOST_CTAS;
     p.k_pitch = ba_pitch(p.a.c.dim);
     p.v_pitch = ba_pitch(p.a.c.vdim);
     p.slab_bytes = ba_slab_bytes(p.k_pitch, p.v_pitch);
-    p.head_bytes = ba_head_bytes(RT, MAXD, p.a.c.vdim, ctas);
+    p.head_bytes = ba_head_bytes(RT, MAXD, p.a.c.vdim / PASSES, ctas);
     const uint32_t smem = p.head_bytes + BA_WARPS * STAGES * p.slab_bytes;
     static thread_local int configured_device = -1;
     if (configured_device != ctx->device) {

@@ -1,4 +1,5 @@
-"""The calls of a serving step at their limits: scores of any size, lengths and block numbers out of range, threads with heads of different sizes."""
+"""The calls of a serving step at their limits: scores of any size, lengths and block numbers out of range, threads with heads of different sizes, results joined in
+passes."""
 from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
@@ -7,6 +8,7 @@ import torch
 
 import hologram_b200 as hb
 from serving_step_reference import HALF_STEP, attend
+from test_serving_step_gpu import test_block_cache_attention as attention_case
 from test_serving_step_gpu import CACHE_WEIGHT_HALF, TORCH, WEIGHT_HALF, Cache, attention, check, f64, packed, starts_of, strided
 
 pytestmark = pytest.mark.gpu
@@ -172,3 +174,17 @@ def test_threads_with_heads_of_different_sizes(large, small, new):
         finally:
             one.submit(first[0].close).result()
             other.submit(second[0].close).result()
+
+
+# ---- eight rows of 128 columns -----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("new,before,block,heads,kv", [
+    ([1] * 40, [(37 * i) % 300 for i in range(40)], 32, 16, 2),      # whole planes, one after another in a CTA
+    ([1, 1, 1], [900, 0, 2500], 16, 12, 2),                          # six rows of eight, parts of planes joined
+    ([2, 3, 1, 0, 4], [70, 5, 640, 3, 1000], 24, 8, 4),
+    ([1], [3999], 64, 8, 1),
+])
+def test_results_of_eight_rows_are_joined_in_two_passes(backend, new, before, block, heads, kv, dtype):
+    attention_case(backend, new, before, block, heads, kv, 128, 128, dtype)
