@@ -58,11 +58,14 @@ class TokenRules:
 
     def __init__(self, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None):
         self.repetition, self.presence, self.frequency = float(repetition), float(presence), float(frequency)
-        if not (0.0 < self.repetition < np.inf and np.isfinite(self.presence) and np.isfinite(self.frequency)):
-            raise ValueError("repetition is positive; repetition, presence and frequency are finite")
         self.bias = {int(t): float(v) for t, v in dict(bias or {}).items()}
-        if any(t < 0 or np.isnan(v) or v == np.inf for t, v in self.bias.items()):
-            raise ValueError("a bias has a token id from 0 on and a finite value, or -inf")
+        # as the device has them, in f32: what is positive or finite here may not be there
+        with np.errstate(over="ignore"):
+            repetition, presence, frequency, *values = np.array([self.repetition, self.presence, self.frequency, *self.bias.values()]).astype(np.float32)
+        if not (0.0 < repetition < np.inf and np.isfinite(presence) and np.isfinite(frequency)):
+            raise ValueError("repetition is positive; repetition, presence and frequency are finite, in f32")
+        if any(t < 0 for t in self.bias) or any(np.isnan(v) or v == np.inf for v in values) or any(v == -np.inf and np.isfinite(b) for v, b in zip(values, self.bias.values())):
+            raise ValueError("a bias has a token id from 0 on and a value that is finite in f32, or -inf")
         self.allowed = allowed if allowed is None or callable(allowed) else self._ids(allowed)
 
     @staticmethod

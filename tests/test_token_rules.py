@@ -15,6 +15,17 @@ def test_rules_without_sense_are_refused(kw):
         dc.TokenRules(**kw)
 
 
+@pytest.mark.parametrize("kw", [{"repetition": 1e-46}, {"repetition": 1e39}, {"presence": 1e39}, {"presence": -1e39}, {"frequency": 1e39}, {"bias": {1: 1e39}}, {"bias": {1: -1e39}}])
+def test_rules_whose_values_f32_does_not_hold_are_refused(kw):
+    with pytest.raises(ValueError):
+        dc.TokenRules(**kw)
+
+
+def test_rules_whose_values_f32_just_holds():
+    r = dc.TokenRules(1e-38, 3e38, -3e38, {0: 3e38, 1: -3e38, 2: -float("inf"), 3: 1e-60})
+    assert (r.repetition, r.presence, r.frequency, r.bias[0], r.bias[2]) == (1e-38, 3e38, -3e38, 3e38, -float("inf"))
+
+
 @pytest.mark.parametrize("vocab", [1, 31, 32, 33, 64, 100])
 def test_masks_have_a_bit_for_each_allowed_token(vocab):
     ids = sorted({0, vocab - 1, vocab // 2})
