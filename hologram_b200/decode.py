@@ -78,11 +78,16 @@ class TokenRules:
     def mask(self, vocab, generated):
         """The allowed tokens as bits of u32 words, or None where all are."""
         ids = self.allowed(list(generated)) if callable(self.allowed) else self.allowed
+        banned = {t for t, v in self.bias.items() if v == -np.inf}
         if ids is None:
+            if len(banned) >= vocab:
+                raise ValueError("the biases leave no token")
             return None
         ids = self._ids(ids)
         if ids.max() >= vocab:
             raise ValueError("an allowed token lies outside the vocabulary")
+        if banned and banned.issuperset(ids.tolist()):
+            raise ValueError("the biases leave none of the allowed tokens")
         bits = np.zeros((vocab + 31) // 32 * 32, dtype=np.uint8)
         bits[ids] = 1
         return np.packbits(bits, bitorder="little").view(np.uint32)

@@ -39,6 +39,19 @@ def test_masks_have_a_bit_for_each_allowed_token(vocab):
         dc.TokenRules(allowed=lambda tokens: []).mask(vocab, [])
 
 
+def test_rules_that_leave_no_token_are_refused():
+    """A step would end with logits of -inf alone, of which a sampler takes a forbidden token."""
+    never = -float("inf")
+    with pytest.raises(ValueError):
+        dc.TokenRules(bias={3: never}, allowed=[3, 3]).mask(8, [])
+    with pytest.raises(ValueError):
+        dc.TokenRules(bias={0: never, 1: never, 2: 1.0}, allowed=lambda tokens: {0, 1}).mask(8, [])
+    with pytest.raises(ValueError):
+        dc.TokenRules(bias={0: never, 1: never}).mask(2, [])
+    assert dc.TokenRules(bias={3: never}, allowed=[3, 4]).mask(8, [])[0] == 0b11000
+    assert dc.TokenRules(bias={0: never}).mask(2, []) is None
+
+
 def test_an_allowing_function_sees_the_generated_tokens():
     rules = dc.TokenRules(allowed=lambda tokens: [len(tokens)])
     assert rules.mask(8, [])[0] == 1 and rules.mask(8, [5, 5, 6])[0] == 8
