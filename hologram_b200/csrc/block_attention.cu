@@ -6,7 +6,7 @@
 // integers, joined in f32. That holds a query to 2^-31 of its row's largest value, whatever its type.
 // Weights: w = 2^(s - max) * scale_v, f32, relative to a power of two that follows the largest scale_v seen and lifted by 2^14, so that weights 2^28
 // below the largest are still normal f16; two f16 terms hold 22 bits. Four rows take both terms in the eight columns of one product; eight rows
-// take two products, or, for a bf16 result, the first term alone (2^-12 of a weight, a sixteenth of the result's own rounding).
+// take two products, or, for a bf16 result, the first term alone (2^-11 of a weight, an eighth of the result's own rounding).
 // Values: a code is exact in f16; two of them take a byte permute onto 1024's exponent and a packed subtraction (1024 + 128 + c - 1152).
 // The product is V^T w^T (m16n8k16): a weight's place among the scores is its place as an operand, nothing is transposed.
 //

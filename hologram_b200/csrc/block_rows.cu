@@ -9,7 +9,7 @@
 // before is worked on, and are the operands of mma.sync m16n8k16 with f32 sums. Query rows are scaled by a power of two to a largest value in
 // [2^14, 2^15), so that bf16 and f16 queries are exact in f16 (values 2^29 smaller than the largest aside); f32 queries go as two f16 terms,
 // which hold 22 bits. Scales of blocks are applied to the scores, and to the weights, w = 2^(s - max) * scale_v relative to a power of two that
-// follows the largest scale_v seen, lifted by 2^14; weights are rounded to f16 (2^-12 of a weight), for an f32 result to two terms.
+// follows the largest scale_v seen, lifted by 2^14; weights are rounded to f16 (by up to 2^-11 of a weight), for an f32 result to two terms.
 // Bound: the rate of mma.sync (8 cycles a product and quarter of an SM), a half of what tcgen05 has; the codes would have to be turned into f16
 // for it as well. The slabs of all planes form one list that the CTAs share out evenly, as for few rows (block_list.cuh).
 #include "block_list.cuh"

@@ -8,7 +8,7 @@
 //   warp 1     tcgen05.mma issuer: S = Q K^T of a tile while the softmax of the one before runs, then O += P V with P read from TMEM
 //   warps 4-7  softmax, one thread per row. A block's scales are the same for 16 keys in a row: the key scale is a factor of the scores, the
 //              value scale a term of the exponent, w = 2^(s - max + log2 scale_v), and is taken out of the row's sum again. Weights are
-//              relative to a power of two above the largest value scale of the CTA's keys and rounded to f16 (2^-12 of a weight)
+//              relative to a power of two above the largest value scale of the CTA's keys and rounded to f16 (by up to 2^-11 of a weight)
 // The tiles of all planes form one list that the CTAs share out evenly; parts of a plane are joined as for few rows (block_list.cuh).
 // TMEM: S of even tiles at 0, of odd ones at 128, their weights over them, O at 256.
 // Bound: the softmax (3700 cycles a tile of 128 x 128, of which 1024 are ex2) and a plane's beginning (12 k cycles: queries, scales, first codes);
@@ -26,7 +26,7 @@ constexpr float BT_GROWTH = 8.0f;
 constexpr int BT_LIFT = 7;
 // A row's maximum (an exponent of two) of this size and more is taken off its scores before the exponents of value scales are added. Below, both
 // are one sum, 2^-13 off at most, and the scores' product with their factor is fused with it; above, that sum loses the scales'
-// exponents and the fused product the rounding that the maximum had, by whole factors of a weight. The test costs 1.5 % (110.0 -> 111.7 us).
+// exponents and the fused product the rounding that the maximum had, by whole factors of a weight. The test costs 1.5 %.
 constexpr float BT_FAR = 0x1p12f;
 
 struct BlockTileParams {

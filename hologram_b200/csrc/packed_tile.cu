@@ -9,8 +9,10 @@
 //              issuer 150 to 300 cycles while the tensor core has the shared memory; two of them hide each other's (8192 rows: 353 -> 311 us)
 //   warps 4-11 softmax, one group of four warps per query tile, one thread per row: running maximum, exponentials, row sum;
 //              a row's O is rescaled in TMEM only when its maximum grows by more than 2^GROWTH
-// The weights are rounded to the operands' type (2^-9 of a weight in bf16, 2^-12 in f16, at most), sums stay f32: a rounded weight moves
-// a result by as much as the result's own rounding does, and a second term for the remainder would be half as many products again.
+// The weights are rounded to the operands' type (by up to 2^-8 of a weight in bf16, 2^-11 in f16), sums stay f32: a rounded weight moves
+// a result by as much as the result's own rounding does, and a second term for the remainder would be half as many products again. Errors
+// against 64 bits are 1.1 to 1.4 times those with f32 weights (8192 rows of bf16 0.0020 against 0.0016 of a result, documents of f16 0.00028
+// against 0.00021).
 // TMEM (512 columns): S at 0 and 128, overwritten by its weights, O at 256 and 384.
 // Bound: two products per score on the tensor core (1024 cycles a 128 x 128 tile at dim 128), and 1024 cycles of ex2 beside it. Measured (32
 // heads over 8 of dim 128, 8192 rows of seven sequences): 275 us, 0.41 of the burst rate of a large bf16 product; a pair of tiles takes

@@ -570,10 +570,12 @@ typedef struct HoloMoeCombineCall {
 
 /* Extension. Attention of whole sequences packed one behind another: sequence s is rows [starts[s], starts[s + 1]) of q, k, v and
  * output (starts i32 [sequences + 1], ascending, from 0 to `rows` at most; empty sequences are allowed). Query head h reads kv head
- * h / (heads / kv_heads). Row i sees the rows j <= i of its sequence (causal) or all of them. Scores and sums are f32:
+ * h / (heads / kv_heads). Row i sees the rows j <= i of its sequence (causal) or all of them:
  *   out[i, h] = sum_j exp(scale q_i . k_j) v_j / sum_j exp(scale q_i . k_j)
  * q [rows, heads * dim] with pitch q_ld, k [rows, kv_heads * dim] with pitch k_ld, v [rows, kv_heads * vdim] with pitch v_ld, output
- * [rows, heads * vdim] with pitch ld, all `dtype` (f32, bf16 or f16; rounded to nearest), dims up to 512. scale_bits 0 selects
+ * [rows, heads * vdim] with pitch ld, all `dtype` (f32, bf16 or f16; rounded to nearest), dims up to 512. Scores and sums are f32; for the
+ * product with v the weights of 16-bit calls may be rounded to `dtype` (by up to 2^-8 of a weight in bf16, 2^-11 in f16: a result then has
+ * up to 1.4 times the error of one with f32 weights; ATTENTION keeps two terms of them). scale_bits 0 selects
  * 1 / sqrt(dim); another scale is positive and finite. Rows of no sequence are left as they were, a row whose scores are all -inf is
  * zero. A row is a function of the rows it sees alone: what stands in others, infinities and NaN included, does not reach it.
  * Starts that descend or leave [0, rows] are reported at the next synchronising call; rows outside any proper range are not stored. */
@@ -611,7 +613,10 @@ typedef struct HoloBlockCacheWriteCall {
 /* Extension. Row i of the n rows of sequence s sees positions j <= lengths[s] - n + i (it is its own last one, written before):
  *   out = sum_j exp(scale q . k_j) v_j / sum_j exp(scale q . k_j)   over the values held, scores and sums f32
  * q [rows, heads * dim] (pitch q_ld), output [rows, heads * vdim] (pitch ld), `dtype` f32, bf16 or f16 (rounded to nearest); dims up to
- * 512; scale_bits as in PACKED_ATTENTION. A row that sees nothing is zero; rows of no sequence are left as they were. */
+ * 512; scale_bits as in PACKED_ATTENTION. For the product with v a weight may be held in f16: in two terms for f32 (2^-21 of a weight), and
+ * for f16 where sequences have few rows; else in one (by up to 2^-11 of a weight, or 2^-25 of the row's largest where that is more).
+ * A row that sees nothing is zero; rows of no sequence are left as they were. The kernel is chosen by the rows a sequence has on average:
+ * single tokens and long portions are answered sooner in a call each than in one. */
 typedef struct HoloBlockCacheAttentionCall {
     HoloBufferRef q, starts, lengths, table, k_codes, k_scales, v_codes, v_scales, output;
     uint32_t rows, sequences, heads, kv_heads, dim, vdim, q_ld, ld, block_rows, blocks, table_ld, scale_bits;
