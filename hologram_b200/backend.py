@@ -137,12 +137,27 @@ class B200Backend:
         self._h = h
         self.device = device
         self._workspaces = weakref.WeakSet()
+        self._natives = {}      # handle of what was made on the context -> what destroys it
+
+    def _keep(self, owner, destroy):
+        """`owner`, whose handle `destroy` takes, lives on this context."""
+        self._workspaces.add(owner)
+        self._natives[owner._h.value] = destroy
+
+    def _destroy(self, handle):
+        """Destroy what has this handle, unless the context was destroyed first and took it along."""
+        destroy = self._natives.pop(handle.value, None)
+        if destroy:
+            destroy(handle)
 
     def close(self):
         """Destroy the context; device workspaces created on it are destroyed first."""
         if getattr(self, "_h", None):
             for ws in list(self._workspaces):
                 ws.close()
+            # the garbage collector clears weak references before it finalises what they named, in any order
+            for handle in reversed(list(self._natives)):
+                self._destroy(C.c_void_p(handle))
             lib.holo_b200_ctx_destroy(self._h)
             self._h = None
 
@@ -223,11 +238,11 @@ class DeviceWorkspace:
         self._h = h
         self.backend = backend
         self.n_slots = n_slots
-        backend._workspaces.add(self)
+        backend._keep(self, lib.holo_b200_workspace_destroy)
 
     def close(self):
         if getattr(self, "_h", None):
-            lib.holo_b200_workspace_destroy(self._h)
+            self.backend._destroy(self._h)
             self._h = None
 
     def __del__(self):
@@ -331,11 +346,14 @@ class DevicePool:
         _check(lib.holo_b200_pool_create(backend._h if backend is not None else None, C.byref(h)))
         self._h, self.backend = h, backend
         if backend is not None:
-            backend._workspaces.add(self)
+            backend._keep(self, lib.holo_b200_pool_destroy)
 
     def close(self):
         if getattr(self, "_h", None):
-            lib.holo_b200_pool_destroy(self._h)
+            if self.backend is not None:
+                self.backend._destroy(self._h)
+            else:
+                lib.holo_b200_pool_destroy(self._h)
             self._h = None
 
     def __del__(self):

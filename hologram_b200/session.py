@@ -134,7 +134,7 @@ class InferenceSession:
         self.addressed = addressed
         self._h = h
         self.backend = backend
-        backend._workspaces.add(self)
+        backend._keep(self, lib.holo_b200_session_destroy)
         ws = DeviceWorkspace.__new__(DeviceWorkspace)
         ws._h, ws.backend, ws.n_slots = vp(lib.holo_b200_session_workspace(h)), backend, None
         ws.close = lambda: None          # owned by the session
@@ -209,7 +209,7 @@ class InferenceSession:
 
     def close(self):
         if getattr(self, "_h", None):
-            lib.holo_b200_session_destroy(self._h)
+            self.backend._destroy(self._h)
             self._h = None
 
     def __del__(self):
